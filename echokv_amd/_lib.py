@@ -26,7 +26,9 @@ EXPORTS = (
     "echokv_gather", "echokv_write_headers",
     "echokv_store_blocks", "echokv_decode", "echokv_decode_static", "echokv_prefill", "echokv_prefill_split",
     "echokv_prefill_dense", "echokv_prefill_dense_workspace", "echokv_prefill_own_group",
-    "echokv_dequant_dense", "echokv_canary_kl", "echokv_decode_workspace_rows",
+    "echokv_dequant_dense", "echokv_canary_kl", "echokv_decode_workspace_rows", "echokv_prompt",
+    "echokv_prompt_tile_m", "echokv_prefix", "echokv_prefix_workspace", "echokv_shared_decode",
+    "echokv_shared_decode_workspace",
 )
 
 
@@ -70,6 +72,14 @@ _SIGS = {
                                  P, P, I64, I64, I32, FL, P],
     "echokv_prefill_dense": [LP, P, P, P, RP, P, I64, I64, I32, I32, P, I64, I64, I32, P, I64, P, I64, I32, P, I64,
                              P, I64, FL, I32, P, P],
+    "echokv_prompt": [P, I64, I64, P, I64, I64, P, I64, I64, I32, I32, I32, I32, P, I64, I32, FL, P, I64, I64, P, P, I64,
+                      I64, I32, P, P],
+    "echokv_prefix": [LP, P, P, P, RP, P, I64, I64, I32, I32, P, I64, P, I64, FL, P, I64, P, I64, I64, P, P],
+    "echokv_shared_decode": [LP, P, P, P, RP, P, I64, I64, I32, I32, P, P, I64, P, P, I64, P, I64, FL, I32, I32, I32, P,
+                             P, I64, P, I64, I64, I32, P],
+    "echokv_prompt_tile_m": [I32, I32, I32],
+    "echokv_prefix_workspace": [LP, I32, I64, I64],
+    "echokv_shared_decode_workspace": [LP, I32, I64, I64, I32],
     "echokv_dequant_dense": [LP, P, P, P, RP, P, I64, P, I64, P, P, I64, I64, I32, P],
     "echokv_canary_kl": [P, I32, I64, I64, I64, P, I64, I64, I64, I32, I32, I32, I32, I32, I32, I32, I32, I32, FL, P, P,
                          P],
@@ -97,6 +107,8 @@ def lib() -> C.CDLL:
         l.echokv_prefill_dense_workspace.restype = C.c_int64
         l.echokv_decode_workspace_rows.argtypes = [LP, I32, I32, I64, I32, I32]
         l.echokv_decode_workspace_rows.restype = C.c_int64
+        l.echokv_prefix_workspace.restype = C.c_int64
+        l.echokv_shared_decode_workspace.restype = C.c_int64
         _lib = l
     return _lib
 
@@ -106,6 +118,14 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib().echokv_error_string(rc).decode()
         raise RuntimeError(f"{name}: {msg} (code {rc})")
+
+
+def size(name: str, *args) -> int:
+    """A count that an entry point returns (a negative one is minus an error code)."""
+    n = int(getattr(lib(), name)(*args))
+    if n < 0:
+        raise ValueError(f"{name}: {lib().echokv_error_string(-n).decode()} (code {-n})")
+    return n
 
 
 def dtype_code(t: torch.Tensor) -> int:
@@ -134,6 +154,14 @@ def require_device(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and t.device.type != "cuda":
             raise RuntimeError(f"EchoKV kernels need device tensors, got a {t.device} tensor")
+
+
+def require_current(*ts: torch.Tensor) -> None:
+    """Device tensors, all on the current device: the launch goes to its current stream."""
+    require_device(*ts)
+    for t in ts:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise RuntimeError(f"tensor on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 def residual(res: torch.Tensor) -> Residual:

@@ -213,14 +213,15 @@ int decode_ps(const ek::DecodeArgs& a, int gqa) {
 }
 
 // echokv_decode and echokv_decode_static: the checks, then decode + merge with
-// the given workspaces, or (static_scratch) with the library's static scratch.
+// the given workspaces, or (static_scratch) with the library's static scratch. With `join`
+// (echokv_shared_decode, split schedule) the splits are left for it to add, as it says.
 int decode_run(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res, const int64_t* res_group,
                const echokv_residual* res, const void* query, int64_t q_s0, int64_t q_s1, int32_t q_dtype,
                int32_t num_q_heads, const int64_t* q_rows, const int32_t* block_table, int64_t bt_s0,
                const int64_t* bt_rows, const int64_t* seq_lens, int64_t num_seqs, float softmax_scale,
                int32_t num_splits, int32_t blocks_per_split, int32_t tier, const int32_t* tier_mask, int32_t flags,
                float* acc, float* ml, bool static_scratch, void* out, int64_t o_s0, int64_t o_s1, int32_t out_dtype,
-               echokv_stream_t stream) {
+               echokv_stream_t stream, ek::JoinArgs* join = nullptr) {
   if (!lay_ok(L)) return ECHOKV_ESHAPE;
   const bool mfma = decode_mfma(L);
   if (!mfma && L->head_size > ek::kMaxAnyD) return ECHOKV_ESHAPE;
@@ -308,6 +309,7 @@ int decode_run(const echokv_layout* L, const uint8_t* pages, const int64_t* bloc
                                 : ek::launch_decode_any(a, (hipStream_t)stream);
       if (d != hipSuccess) return ECHOKV_ELAUNCH;
     }
+    if (join) continue;
     hipError_t e;
     if (a.ranges > 0) {
       e = ek::launch_merge_balanced(a, (hipStream_t)stream);
@@ -317,6 +319,12 @@ int decode_run(const echokv_layout* L, const uint8_t* pages, const int64_t* bloc
       e = mfma ? ek::launch_merge(m, num_seqs, (hipStream_t)stream) : ek::launch_merge_any(m, (hipStream_t)stream);
     }
     if (e != hipSuccess) return ECHOKV_ELAUNCH;
+  }
+  if (join) {
+    join->acc = acc;
+    join->ml = ml;
+    join->sp = a.sp;
+    return launched(ek::launch_join(*join, (hipStream_t)stream));
   }
   return ECHOKV_OK;
 }
@@ -587,6 +595,196 @@ int echokv_prefill_own_group(const echokv_layout* L, const uint8_t* pages, const
   a.out_dtype = out_dtype;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   return launched(ek::launch_own_group(a, n_rows, (hipStream_t)stream));
+}
+
+int32_t echokv_prompt_tile_m(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_size) {
+  if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return -ECHOKV_ESHAPE;
+  if (head_size <= 0 || head_size % 4 || head_size > ek::kMaxAnyD) return -ECHOKV_ESHAPE;
+  const int rows = ek::kPromptRows / (num_q_heads / num_kv_heads);
+  return rows < 1 ? 1 : rows;
+}
+
+int echokv_prompt(const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0, int64_t k_s1,
+                  const void* value, int64_t v_s0, int64_t v_s1, int32_t dtype, int32_t num_q_heads,
+                  int32_t num_kv_heads, int32_t head_size, const int32_t* tiles, int64_t n_tiles, int32_t tile_m,
+                  float softmax_scale, const float* part, int64_t p_s0, int64_t p_s1, const float* part_lse,
+                  void* out, int64_t o_s0, int64_t o_s1, int32_t out_dtype, float* lse, echokv_stream_t stream) {
+  const int32_t rows = echokv_prompt_tile_m(num_q_heads, num_kv_heads, head_size);
+  if (rows < 0) return -rows;
+  if (tile_m != rows) return ECHOKV_ESHAPE;
+  if (!dtype_ok(dtype) || !dtype_ok(out_dtype)) return ECHOKV_EDTYPE;
+  if (n_tiles < 0 || n_tiles > INT32_MAX / num_kv_heads || (part && !part_lse)) return ECHOKV_EINVAL;
+  if (n_tiles == 0) return ECHOKV_OK;
+  if (!query || !key || !value || !tiles || !out) return ECHOKV_EINVAL;
+  ek::PromptArgs a;
+  a.q = query;
+  a.q_s0 = q_s0;
+  a.q_s1 = q_s1;
+  a.k = key;
+  a.k_s0 = k_s0;
+  a.k_s1 = k_s1;
+  a.v = value;
+  a.v_s0 = v_s0;
+  a.v_s1 = v_s1;
+  a.dtype = dtype;
+  a.hq = num_q_heads;
+  a.H = num_kv_heads;
+  a.gqa = num_q_heads / num_kv_heads;
+  a.D = head_size;
+  a.tiles = tiles;
+  a.n_tiles = (int)n_tiles;
+  a.tile_m = tile_m;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.part = part;
+  a.p_s0 = p_s0;
+  a.p_s1 = p_s1;
+  a.part_lse = part_lse;
+  a.out = out;
+  a.o_s0 = o_s0;
+  a.o_s1 = o_s1;
+  a.out_dtype = out_dtype;
+  a.lse = lse;
+  return launched(ek::launch_prompt_any(a, (hipStream_t)stream));
+}
+
+}  // extern "C"
+
+namespace {
+
+// Ranges of a shared prefix: enough workgroups for the chip (two for each of its 256
+// CUs) with at least 128 keys each.
+int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
+  const int64_t gqa = hq / L->num_kv_heads, wgs = (n * gqa + 63) / 64 * L->num_kv_heads;
+  int64_t r = (512 + wgs - 1) / wgs;
+  const int64_t most = len / 128;
+  r = r < most ? r : most;
+  return (int)(r < 1 ? 1 : r < 64 ? r : 64);
+}
+
+bool prefix_shape_ok(const echokv_layout* L, int hq, int64_t n, int64_t len) {
+  if (!lay_ok(L) || L->head_size > ek::kMaxAnyD || hq <= 0 || hq % L->num_kv_heads) return false;
+  // Grids: (rows / 64) x heads x ranges workgroups, rows / 4 waves of the join.
+  return n >= 0 && n <= INT32_MAX / 64 / hq && len >= 0 && len <= INT32_MAX - 1024;
+}
+
+// Float32 rows of `hq` heads and their (max, sum) pairs, behind one another.
+int64_t rows_bytes(int64_t rows, int D) { return rows * (D + 2) * 4; }
+
+// The shared part of echokv_prefix and echokv_shared_decode; n > 0 and the shapes checked.
+ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,
+                           const int64_t* res_group, const echokv_residual* res, const void* query, int64_t q_s0,
+                           int64_t q_s1, int32_t q_dtype, int32_t hq, const int64_t* q_rows, int64_t n,
+                           const int32_t* blocks, int64_t len, float softmax_scale, int ranges, void* workspace) {
+  ek::PrefixArgs a;
+  a.L = to_lay(L);
+  a.pages = pages;
+  a.block_res = block_res;
+  a.res_group = res_group;
+  a.res = to_res(res);
+  a.q = query;
+  a.q_s0 = q_s0;
+  a.q_s1 = q_s1;
+  a.q_dtype = q_dtype;
+  a.hq = hq;
+  a.gqa = hq / L->num_kv_heads;
+  a.q_rows = q_rows;
+  a.n = n;
+  a.blocks = blocks;
+  a.len = (int)len;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.ranges = ranges;
+  a.per = (int)((len + ranges - 1) / ranges + 63) / 64 * 64;
+  a.acc = (float*)workspace;
+  a.ml = a.acc + ranges * n * hq * L->head_size;
+  a.part = nullptr;
+  a.p_s0 = a.p_s1 = 0;
+  a.lse = nullptr;
+  a.lens = nullptr;
+  a.suffix = nullptr;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t n, int64_t prefix_len) {
+  if (!prefix_shape_ok(L, num_q_heads, n, prefix_len)) return -ECHOKV_ESHAPE;
+  if (n == 0) return 0;
+  const int64_t ranges = prefix_ranges(L, num_q_heads, n, prefix_len);
+  return ranges > 1 ? rows_bytes(ranges * n * num_q_heads, L->head_size) : 0;
+}
+
+int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res, const int64_t* res_group,
+                  const echokv_residual* res, const void* query, int64_t q_s0, int64_t q_s1, int32_t q_dtype,
+                  int32_t num_q_heads, const int64_t* q_rows, int64_t n, const int32_t* blocks, int64_t prefix_len,
+                  float softmax_scale, void* workspace, int64_t workspace_bytes, float* part, int64_t p_s0,
+                  int64_t p_s1, float* lse, echokv_stream_t stream) {
+  const int64_t need = echokv_prefix_workspace(L, num_q_heads, n, prefix_len);
+  if (need < 0) return (int)-need;
+  if (!dtype_ok(q_dtype)) return ECHOKV_EDTYPE;
+  if (!res_ok(res)) return ECHOKV_EINVAL;
+  if (n == 0) return ECHOKV_OK;
+  if (!pages || !block_res || !res_group || !query || !part || !lse || (prefix_len > 0 && !blocks)) return ECHOKV_EINVAL;
+  if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return ECHOKV_EINVAL;
+  const int ranges = prefix_ranges(L, num_q_heads, n, prefix_len);
+  ek::PrefixArgs a = prefix_args(L, pages, block_res, res_group, res, query, q_s0, q_s1, q_dtype, num_q_heads, q_rows,
+                                 n, blocks, prefix_len, softmax_scale, ranges, workspace);
+  if (ranges == 1) {
+    a.part = part;
+    a.p_s0 = p_s0;
+    a.p_s1 = p_s1;
+    a.lse = lse;
+    return launched(ek::launch_prefix_any(a, (hipStream_t)stream));
+  }
+  if (ek::launch_prefix_any(a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
+  const ek::JoinArgs j{a.acc, a.ml, ranges, nullptr, nullptr, nullptr, 0, ek::Splits{}, nullptr, 0, L->block_size,
+                       q_rows, n, num_q_heads, L->head_size, part, p_s0, p_s1, ECHOKV_F32, lse};
+  return launched(ek::launch_join(j, (hipStream_t)stream));
+}
+
+int64_t echokv_shared_decode_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t num_seqs,
+                                       int64_t prefix_len, int32_t num_splits) {
+  if (!prefix_shape_ok(L, num_q_heads, num_seqs, prefix_len)) return -ECHOKV_ESHAPE;
+  if (num_splits <= 0 || num_splits > (1 << 20)) return -ECHOKV_EINVAL;
+  if (num_seqs == 0) return 0;
+  const int64_t ranges = prefix_ranges(L, num_q_heads, num_seqs, prefix_len);
+  return (num_seqs * 8 + 15) / 16 * 16 + rows_bytes((ranges + num_splits) * num_seqs * num_q_heads, L->head_size);
+}
+
+int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,
+                         const int64_t* res_group, const echokv_residual* res, const void* query, int64_t q_s0,
+                         int64_t q_s1, int32_t q_dtype, int32_t num_q_heads, const int64_t* q_rows,
+                         const int32_t* block_table, int64_t bt_s0, const int64_t* bt_rows, const int64_t* seq_lens,
+                         int64_t num_seqs, const int32_t* blocks, int64_t prefix_len, float softmax_scale,
+                         int32_t num_splits, int32_t blocks_per_split, int32_t tier, const int32_t* tier_mask,
+                         void* workspace, int64_t workspace_bytes, void* out, int64_t o_s0, int64_t o_s1,
+                         int32_t out_dtype, echokv_stream_t stream) {
+  const int64_t need = echokv_shared_decode_workspace(L, num_q_heads, num_seqs, prefix_len, num_splits);
+  if (need < 0) return (int)-need;
+  if (prefix_len == 0 || prefix_len % L->block_size) return ECHOKV_EINVAL;
+  if (!dtype_ok(q_dtype) || !dtype_ok(out_dtype)) return ECHOKV_EDTYPE;
+  if (blocks_per_split <= 0 || (tier != 2 && tier != 4 && tier != 8) || !res_ok(res)) return ECHOKV_EINVAL;
+  if (num_seqs == 0) return ECHOKV_OK;
+  if (!pages || !block_res || !res_group || !query || !block_table || !seq_lens || !blocks || !out) return ECHOKV_EINVAL;
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) return ECHOKV_EINVAL;
+  const int ranges = prefix_ranges(L, num_q_heads, num_seqs, prefix_len);
+  int64_t* suffix = (int64_t*)workspace;
+  float* rows = (float*)((uint8_t*)workspace + (num_seqs * 8 + 15) / 16 * 16);
+  ek::PrefixArgs a = prefix_args(L, pages, block_res, res_group, res, query, q_s0, q_s1, q_dtype, num_q_heads, q_rows,
+                                 num_seqs, blocks, prefix_len, softmax_scale, ranges, rows);
+  a.lens = seq_lens;
+  a.suffix = suffix;
+  if (ek::launch_prefix_any(a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
+  float* acc = rows + ranges * num_seqs * num_q_heads * (L->head_size + 2);
+  float* ml = acc + num_splits * num_seqs * num_q_heads * L->head_size;
+  ek::JoinArgs j{a.acc, a.ml, ranges, nullptr, nullptr, suffix, num_splits, ek::Splits{}, seq_lens, (int)prefix_len,
+                 L->block_size, q_rows, num_seqs, num_q_heads, L->head_size, out, o_s0, o_s1, out_dtype, nullptr};
+  const int32_t flags = ECHOKV_DECODE_BATCH_INVARIANT | (num_splits >= 4 ? ECHOKV_DECODE_SHORT_SPLITS : 0);
+  return decode_run(L, pages, block_res, res_group, res, query, q_s0, q_s1, q_dtype, num_q_heads, q_rows,
+                    block_table + prefix_len / L->block_size, bt_s0, bt_rows, suffix, num_seqs, softmax_scale,
+                    num_splits, blocks_per_split, tier, tier_mask, flags, acc, ml, false, out, o_s0, o_s1, out_dtype,
+                    stream, &j);
 }
 
 int echokv_dequant_dense(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,

@@ -354,6 +354,84 @@ struct FlashArgs {
   int hq;
 };
 
+// ---- whole prompts (prompt.hip) and a shared cached prefix (shared.hip) --------
+
+// Causal attention of packed prompts over their own keys and values: query row t of a
+// sequence sees key rows [first row, t]. Rows of a tile are (token, GQA head) pairs.
+constexpr int kPromptRows = 256;     // query rows of a tile
+struct PromptArgs {
+  const void* q;
+  long q_s0, q_s1;
+  const void* k;
+  long k_s0, k_s1;
+  const void* v;
+  long v_s0, v_s1;
+  int dtype, hq, H, gqa, D;
+  const int32_t* tiles;  // [n, 4]: the sequence's first row, its tokens, the tile's first token, its tokens
+  int n_tiles, tile_m;
+  float scale_log2;
+  // Nullable: attention of the same query rows over keys before the prompt, joined with the
+  // result: normalized float32 rows and their log2-domain log-sum-exp [rows, hq] (-inf: none).
+  const float* part;
+  long p_s0, p_s1;
+  const float* part_lse;
+  void* out;
+  long o_s0, o_s1;
+  int out_dtype;
+  float* lse;  // nullable: [rows, hq]
+};
+
+// Attention of every query row over the same `len` cached keys (blocks: their block list), cut
+// into `ranges` of `per` keys. Range z of query row t and head qh leaves its unnormalized
+// output and (max in log2 units, sum) in row (z * n + t) * hq + qh of acc [.., D] and
+// ml [.., 2]; with ranges == 1 and part set the normalized row and its log-sum-exp instead.
+struct PrefixArgs {
+  Lay L;
+  const uint8_t* pages;
+  const int64_t* block_res;
+  const int64_t* res_group;
+  Res res;
+  const void* q;
+  long q_s0, q_s1;
+  int q_dtype, hq, gqa;
+  const int64_t* q_rows;  // nullable: query row of entry t (t itself)
+  long n;                 // entries
+  const int32_t* blocks;
+  int len;
+  float scale_log2;
+  int ranges, per;
+  float* acc;
+  float* ml;
+  float* part;
+  long p_s0, p_s1;
+  float* lse;
+  // Decode: suffix[t] = the tokens of sequence t behind the prefix (0 where it is shorter),
+  // written for the kernels that follow.
+  const int64_t* lens;
+  int64_t* suffix;
+};
+
+// The ranges of the prefix and, in decode, the splits of the suffixes, added and normalized.
+struct JoinArgs {
+  const float* p_acc;
+  const float* p_ml;
+  int ranges;
+  const float* acc;  // suffix splits (null: none), as DecodeArgs::acc / ml with their lengths
+  const float* ml;
+  const int64_t* suffix;
+  int num_splits;
+  Splits sp;
+  const int64_t* lens;  // nullable: entries shorter than `len` leave their row as it is
+  int len, BS;
+  const int64_t* q_rows;
+  long n;
+  int hq, D;
+  void* out;
+  long o_s0, o_s1;
+  int out_dtype;
+  float* lse;  // nullable: [rows, hq]
+};
+
 // Raise `kernel`'s dynamic-LDS limit to `bytes` on the current device, once per
 // device. The flag only skips a repeated call: hipFuncSetAttribute is idempotent,
 // so two threads that race on a fresh device both make it and both succeed.
@@ -404,5 +482,8 @@ size_t canary_lds_bytes(int d, int nbits, int kg);  // one canary workgroup's LD
 hipError_t launch_prefill(const PrefillArgs& a, long n, long n_merges, hipStream_t s);
 hipError_t launch_prefill_pack(const PackArgs& a, long n_packs, hipStream_t s);
 hipError_t launch_prefill_flash(const FlashArgs& a, hipStream_t s);
+hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s);
+hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s);
+hipError_t launch_join(const JoinArgs& a, hipStream_t s);
 
 }  // namespace ek

@@ -1,0 +1,382 @@
+// Attention over whole prompts and over a shared cached prefix in 32-bit arithmetic, for
+// any head size that is a multiple of 4 (up to 256), any types, strides and alignment.
+//
+// A workgroup holds 64 query rows ((token, GQA head) pairs of one KV head), 16 per wave. The
+// keys come in steps of 32 (16 at head sizes above 128), staged in LDS as float32 -- from the
+// prompt's own rows, or dequantized from the cache's pages -- and each wave runs
+//   S^T[key, row] = K Q^T         (v_mfma_f32_16x16x4_f32)
+//   O^T[d, row]  += V^T P^T       (v_mfma_f32_16x16x4_f32)
+// with an online softmax per row. A contraction index may be permuted as long as both
+// operands are: lane group c takes channels 16 j + 4 c .. + 4 of the score products (one
+// 16-byte read each), and keys 4 c + i of the value products, which is where the S^T
+// accumulator holds them, so P^T needs no exchange.
+//
+// Bound by the float32 matrix rate (1/16 of the 16-bit one) on long prompts.
+#include "items.h"
+
+namespace ek {
+namespace {
+
+constexpr int kRows = 64;  // query rows per workgroup
+constexpr float kInf = __builtin_inff();
+
+template <int DP>
+struct Steps {
+  static constexpr int KEYS = DP > 128 ? 16 : 32;
+  static constexpr int PITCH = DP + 4;  // floats per LDS row: 16 rows' 16-byte reads spread over the banks
+  static constexpr int NKH = KEYS / 16, NJ = DP / 16;
+};
+
+__device__ __forceinline__ float rows_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+
+__device__ __forceinline__ bool finite4(const float* x) {
+  // An exponent of all ones somewhere.
+  uint32_t bad = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bad |= (__float_as_uint(x[e]) & 0x7f800000u) == 0x7f800000u;
+  return !bad;
+}
+
+// One wave's 16 rows: accumulators O^T (lane (n, c): row n, channels 16 j + 4 c + i), the
+// running max (log2 units) and this lane's share of the sum.
+template <int DP>
+struct State {
+  f4_t acc[Steps<DP>::NJ];
+  float m, l;
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int j = 0; j < Steps<DP>::NJ; ++j) acc[j] = f4_t{0.f, 0.f, 0.f, 0.f};
+    m = -kInf;
+    l = 0.f;
+  }
+};
+
+// A step of KEYS staged keys, the first at position kb: a row sees keys below its `lim`.
+// `odd`: a value of the step is infinite or NaN, which a weight of zero must not reach.
+template <int DP>
+__device__ __forceinline__ void step_any(State<DP>& st, const f4_t* q, const float* kt, const float* vt, int kb,
+                                         int lim, bool odd, int lane) {
+  using S = Steps<DP>;
+  const int n = lane & 15, c = lane >> 4;
+  f4_t s[S::NKH];
+#pragma unroll
+  for (int kh = 0; kh < S::NKH; ++kh) s[kh] = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < S::NJ; ++j) {
+#pragma unroll
+    for (int kh = 0; kh < S::NKH; ++kh) {
+      const f4_t k = *(const f4_t*)&kt[(16 * kh + n) * S::PITCH + 16 * j + 4 * c];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[kh] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[j][e], s[kh], 0, 0, 0);
+    }
+  }
+  float mt = -kInf;
+#pragma unroll
+  for (int kh = 0; kh < S::NKH; ++kh)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = kb + 16 * kh + 4 * c + i < lim ? s[kh][i] : -kInf;
+      s[kh][i] = x;
+      mt = fmaxf(mt, x);
+    }
+  mt = rows_max(mt);
+  if (mt > st.m) {
+    const float alpha = __builtin_amdgcn_exp2f(st.m - mt);
+    st.l *= alpha;
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j) st.acc[j] *= alpha;
+    st.m = mt;
+  }
+  const float ms = st.m == -kInf ? 0.f : st.m;
+#pragma unroll
+  for (int kh = 0; kh < S::NKH; ++kh)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[kh][i] = __builtin_amdgcn_exp2f(s[kh][i] - ms);
+      st.l += s[kh][i];
+    }
+  if (!odd) {
+#pragma unroll
+    for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+      for (int kh = 0; kh < S::NKH; ++kh)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          st.acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(vt[(16 * kh + 4 * c + i) * S::PITCH + 16 * j + n], s[kh][i],
+                                                           st.acc[j], 0, 0, 0);
+    return;
+  }
+  // Rare: key by key, only where the row sees the key.
+#pragma unroll
+  for (int kh = 0; kh < S::NKH; ++kh)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll 1
+      for (int g = 0; g < 4; ++g) {
+        const int key = 16 * kh + 4 * g + i;
+        const float p = __shfl(s[kh][i], 16 * g + n, 64);
+        if (kb + key >= lim) continue;
+#pragma unroll
+        for (int j = 0; j < S::NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            st.acc[j][e] = __builtin_fmaf(p, vt[key * S::PITCH + 16 * j + 4 * c + e], st.acc[j][e]);
+      }
+}
+
+// The row's query, times the softmax scale in log2 units (zeros past the head).
+template <int DP>
+__device__ __forceinline__ void load_q(const void* q, int dtype, long at, int D, float scale, int c, f4_t* x) {
+#pragma unroll
+  for (int j = 0; j < Steps<DP>::NJ; ++j) {
+    const int ch = 16 * j + 4 * c;
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    if (ch < D) ld4(q, dtype, at + ch, y);
+    x[j] = f4_t{y[0] * scale, y[1] * scale, y[2] * scale, y[3] * scale};
+  }
+}
+
+}  // namespace
+
+// One workgroup per (tile, 64 of its rows, KV head); heads fastest.
+template <int DP>
+__global__ __launch_bounds__(256) void prompt_any_kernel(PromptArgs a) {
+  using S = Steps<DP>;
+  __shared__ __attribute__((aligned(16))) float kt[S::KEYS * S::PITCH], vt[S::KEYS * S::PITCH];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, c = lane >> 4;
+  const int h = (int)(blockIdx.x % a.H);
+  const int32_t* td = a.tiles + 4 * (long)(blockIdx.x / a.H);
+  const long row0 = td[0];
+  const int seq = td[1], t0 = td[2], n_rows = td[3] * a.gqa;
+  const int first = (int)blockIdx.y * kRows;
+  if (first >= n_rows) return;
+  const int last = min(first + kRows, n_rows) - 1;
+  const int kv_end = min(seq, t0 + last / a.gqa + 1);  // keys that any row sees
+  const int r = first + 16 * (tid >> 6) + n;
+  const bool live = r < n_rows;
+  const int tok = t0 + (live ? r / a.gqa : 0), qh = h * a.gqa + (live ? r % a.gqa : 0);
+  const int lim = live ? tok + 1 : 0;
+  f4_t q[S::NJ];
+  load_q<DP>(a.q, a.dtype, (row0 + tok) * a.q_s0 + (long)qh * a.q_s1, a.D, a.scale_log2, c, q);
+  State<DP> st;
+  st.init();
+  for (int kb = 0; kb < kv_end; kb += S::KEYS) {
+    __syncthreads();
+    bool odd = false;
+    for (int i = tid; i < S::KEYS * (DP / 4); i += 256) {
+      const int key = i / (DP / 4), ch = 4 * (i % (DP / 4));
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (kb + key < kv_end && ch < a.D) {
+        const long row = row0 + kb + key;
+        ld4(a.k, a.dtype, row * a.k_s0 + (long)h * a.k_s1 + ch, x);
+        ld4(a.v, a.dtype, row * a.v_s0 + (long)h * a.v_s1 + ch, y);
+        odd = odd || !finite4(y);
+      }
+      *(f4_t*)&kt[key * S::PITCH + ch] = f4_t{x[0], x[1], x[2], x[3]};
+      *(f4_t*)&vt[key * S::PITCH + ch] = f4_t{y[0], y[1], y[2], y[3]};
+    }
+    const int any_odd = __syncthreads_or(odd);
+    step_any<DP>(st, q, kt, vt, kb, lim, any_odd != 0, lane);
+  }
+  float l = st.l + __shfl_xor(st.l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (!live) return;
+  const long row = row0 + tok, lr = row * a.hq + qh;
+  float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -kInf : st.m + __log2f(l), wp = 0.f;
+  if (a.part) {
+    const float pl = a.part_lse[lr], top = fmaxf(pl, lse);
+    if (top != -kInf) {
+      const float ep = __builtin_amdgcn_exp2f(pl - top), eo = __builtin_amdgcn_exp2f(lse - top), sum = ep + eo;
+      wp = ep / sum;
+      inv *= eo / sum;
+      lse = top + __log2f(sum);
+    }
+  }
+  if (a.lse && c == 0) a.lse[lr] = lse;
+#pragma unroll
+  for (int j = 0; j < S::NJ; ++j) {
+    const int ch = 16 * j + 4 * c;
+    if (ch >= a.D) continue;
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = st.acc[j][e] * inv;
+    if (wp != 0.f) {
+      const float* p = a.part + row * a.p_s0 + (long)qh * a.p_s1 + ch;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += wp * p[e];
+    }
+    st_n<4>(a.out, a.out_dtype, row * a.o_s0 + (long)qh * a.o_s1 + ch, y);
+  }
+}
+
+// One workgroup per (64 rows, KV head, range); heads fastest, then ranges.
+template <int DP>
+__global__ __launch_bounds__(256) void prefix_any_kernel(PrefixArgs a) {
+  using S = Steps<DP>;
+  __shared__ __attribute__((aligned(16))) float kt[S::KEYS * S::PITCH], vt[S::KEYS * S::PITCH];
+  const Lay& L = a.L;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, c = lane >> 4;
+  if (a.suffix)
+    for (long t = (long)blockIdx.x * 256 + tid; t < a.n; t += (long)gridDim.x * 256) {
+      const long x = a.lens[t] - a.len;
+      a.suffix[t] = x > 0 ? x : 0;
+    }
+  const int h = (int)(blockIdx.x % L.H);
+  const int z = (int)(blockIdx.x / L.H % a.ranges);
+  const long r = blockIdx.x / L.H / a.ranges * kRows + 16 * (tid >> 6) + n;
+  const bool live = r < a.n * a.gqa;
+  const long t = live ? r / a.gqa : 0;
+  const int qh = h * a.gqa + (live ? (int)(r % a.gqa) : 0);
+  const long q_row = a.q_rows ? a.q_rows[t] : t;
+  const int k_begin = z * a.per, k_end = z == a.ranges - 1 ? a.len : min(a.len, k_begin + a.per);
+  f4_t q[S::NJ];
+  load_q<DP>(a.q, a.q_dtype, q_row * a.q_s0 + (long)qh * a.q_s1, L.D, a.scale_log2, c, q);
+  State<DP> st;
+  st.init();
+  constexpr int OCTS = DP / 8;
+  for (int kb = k_begin; kb < k_end; kb += S::KEYS) {
+    __syncthreads();
+    for (int i = tid; i < S::KEYS / 4 * OCTS; i += 256) {
+      const int quad = i / OCTS, ch = 8 * (i % OCTS), kp = kb + 4 * quad;
+      float x[4][8] = {}, y[4][8] = {};
+      if (kp < k_end && ch < L.D) {
+        const long blk = a.blocks[kp / L.BS];
+        if (blk >= 0 && blk < L.nb) {
+          const int off = kp % L.BS, live_keys = k_end - kp;
+          const Hdr hd = load_hdr(a.pages, L, blk);
+          const int bits = tier_of(hd.tag);
+          const long rs = a.block_res[blk];
+          const int rg = (unsigned long)rs < (unsigned long)a.res.rows ? (int)a.res_group[rs] : -1;
+          item_general<true>(L, a.pages, a.res, blk, hd, rs, rg, off, bits, live_keys, h, ch, x);
+          item_general<false>(L, a.pages, a.res, blk, hd, rs, rg, off, bits, live_keys, h, ch, y);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int at = (4 * quad + k) * S::PITCH + ch;
+        *(f4_t*)&kt[at] = f4_t{x[k][0], x[k][1], x[k][2], x[k][3]};
+        *(f4_t*)&kt[at + 4] = f4_t{x[k][4], x[k][5], x[k][6], x[k][7]};
+        *(f4_t*)&vt[at] = f4_t{y[k][0], y[k][1], y[k][2], y[k][3]};
+        *(f4_t*)&vt[at + 4] = f4_t{y[k][4], y[k][5], y[k][6], y[k][7]};
+      }
+    }
+    __syncthreads();
+    step_any<DP>(st, q, kt, vt, kb, k_end, false, lane);
+  }
+  float l = st.l + __shfl_xor(st.l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (!live) return;
+  const bool direct = a.part != nullptr;
+  const long pr = ((long)z * a.n + t) * a.hq + qh;
+  const float inv = !direct ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+  if (c == 0) {
+    if (direct) a.lse[q_row * a.hq + qh] = l == 0.f ? -kInf : st.m + __log2f(l);
+    else *(float2*)(a.ml + 2 * pr) = float2{st.m, l};
+  }
+  float* dst = direct ? a.part + q_row * a.p_s0 + (long)qh * a.p_s1 : a.acc + pr * L.D;
+#pragma unroll
+  for (int j = 0; j < S::NJ; ++j) {
+    const int ch = 16 * j + 4 * c;
+    if (ch >= L.D) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dst[ch + e] = st.acc[j][e] * inv;
+  }
+}
+
+// One wave per (entry, query head): its prefix ranges, then its suffix splits, 64 pieces at a
+// time, the rows of 8 requested together. Lane l takes channels l, l + 64, ...
+template <int C>
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);  // entry * hq + head
+  if (row >= a.n * a.hq) return;
+  const long t = row / a.hq;
+  const int qh = (int)(row % a.hq), D = a.D;
+  if (a.lens && a.lens[t] < a.len) return;
+  int pieces = a.ranges;
+  if (a.acc) {
+    const int nb = ((int)a.suffix[t] + a.BS - 1) / a.BS;
+    if (nb > 0) {
+      const int bps = split_blocks(a.sp, nb);
+      pieces += (nb + bps - 1) / bps;
+    }
+  }
+  // Piece i's row of its workspace.
+  auto at = [&](int i) { return i < a.ranges ? (long)i * a.n * a.hq + row : row * a.num_splits + (i - a.ranges); };
+  float m = -kInf, den = 0.f, o[C] = {};
+  for (int p0 = 0; p0 < pieces; p0 += 64) {
+    float2 x = float2{-kInf, 0.f};
+    if (p0 + lane < pieces) {
+      const int i = p0 + lane;
+      x = *(const float2*)((i < a.ranges ? a.p_ml : a.ml) + 2 * at(i));
+    }
+    float mt = x.x;
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) mt = fmaxf(mt, __shfl_xor(mt, k, 64));
+    const float top = fmaxf(m, mt);
+    if (top == -kInf) continue;
+    const float w = x.x == -kInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
+    float d = w * x.y;
+#pragma unroll
+    for (int k = 32; k > 0; k >>= 1) d += __shfl_xor(d, k, 64);
+    const float alpha = __builtin_amdgcn_exp2f(m - top);
+    den = den * alpha + d;
+#pragma unroll
+    for (int e = 0; e < C; ++e) o[e] *= alpha;
+    m = top;
+    const int last = min(pieces, p0 + 64);
+    for (int i0 = p0; i0 < last; i0 += 8) {
+      float y[8][C];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u < last ? i0 + u : p0;
+        const float* src = (i < a.ranges ? a.p_acc : a.acc) + at(i) * D;
+#pragma unroll
+        for (int e = 0; e < C; ++e) y[u][e] = lane + 64 * e < D ? src[lane + 64 * e] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (i0 + u >= last) continue;
+        const float wu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i0 + u - p0));
+        if (wu == 0.f) continue;  // an empty piece
+#pragma unroll
+        for (int e = 0; e < C; ++e) o[e] = __builtin_fmaf(wu, y[u][e], o[e]);
+      }
+    }
+  }
+  const long q_row = a.q_rows ? a.q_rows[t] : t;
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  if (a.lse && lane == 0) a.lse[q_row * a.hq + qh] = den == 0.f ? -kInf : m + __log2f(den);
+#pragma unroll
+  for (int e = 0; e < C; ++e)
+    if (lane + 64 * e < D) st(a.out, a.out_dtype, q_row * a.o_s0 + (long)qh * a.o_s1 + lane + 64 * e, o[e] * inv);
+}
+
+hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((long)a.n_tiles * a.H), (unsigned)(((long)a.tile_m * a.gqa + kRows - 1) / kRows));
+  if (a.D <= 64) hipLaunchKernelGGL(prompt_any_kernel<64>, grid, dim3(256), 0, s, a);
+  else if (a.D <= 128) hipLaunchKernelGGL(prompt_any_kernel<128>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(prompt_any_kernel<256>, grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.n * a.gqa + kRows - 1) / kRows * a.L.H * a.ranges));
+  if (a.L.D <= 64) hipLaunchKernelGGL(prefix_any_kernel<64>, grid, dim3(256), 0, s, a);
+  else if (a.L.D <= 128) hipLaunchKernelGGL(prefix_any_kernel<128>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(prefix_any_kernel<256>, grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_join(const JoinArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.n * a.hq + 3) / 4));
+  if (a.D <= 64) hipLaunchKernelGGL(join_kernel<1>, grid, dim3(256), 0, s, a);
+  else if (a.D <= 128) hipLaunchKernelGGL(join_kernel<2>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(join_kernel<4>, grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace ek

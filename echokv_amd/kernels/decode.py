@@ -48,6 +48,24 @@ def workspace_rows(store, num_q_heads: int, q_dtype: torch.dtype, num_seqs: int,
     return int(rows)
 
 
+def tier_mask_of(store, tier_mask: torch.Tensor | str | None, device, batch_invariant: bool = True):
+    """``decode_attention``'s ``tier_mask`` argument as the kernels take it: a device word or None."""
+    if isinstance(tier_mask, str):
+        if tier_mask != "auto":
+            raise ValueError(f"tier_mask must be an int32 device tensor or 'auto', got {tier_mask!r}")
+        live = store.pool.live_tiers()
+        present = [b for b in (2, 4, 8) if live[b]]
+        tier_mask = None
+        if len(present) > 1:
+            tier_mask = torch.tensor([sum(present)], dtype=torch.int32, device=device)
+    if tier_mask is not None:
+        if not batch_invariant:
+            raise ValueError("tier passes run on the split schedule: pass batch_invariant=True with tier_mask")
+        if tier_mask.dtype != torch.int32 or tier_mask.device != device or tier_mask.numel() < 1:
+            raise ValueError("tier_mask must be an int32 tensor on the query's device")
+    return tier_mask
+
+
 def decode_attention(
     store,
     query: torch.Tensor,
@@ -141,19 +159,7 @@ def decode_attention(
             raise ValueError(f"decode workspace holds fewer than the {rows} rows this call needs")
         else:
             acc, ml = workspace
-    if isinstance(tier_mask, str):
-        if tier_mask != "auto":
-            raise ValueError(f"tier_mask must be an int32 device tensor or 'auto', got {tier_mask!r}")
-        live = store.pool.live_tiers()
-        present = [b for b in (2, 4, 8) if live[b]]
-        tier_mask = None
-        if len(present) > 1:
-            tier_mask = torch.tensor([sum(present)], dtype=torch.int32, device=dev)
-    if tier_mask is not None:
-        if not batch_invariant:
-            raise ValueError("tier passes run on the split schedule: pass batch_invariant=True with tier_mask")
-        if tier_mask.dtype != torch.int32 or tier_mask.device != dev or tier_mask.numel() < 1:
-            raise ValueError("tier_mask must be an int32 tensor on the query's device")
+    tier_mask = tier_mask_of(store, tier_mask, dev, batch_invariant)
     if tier is None:
         tier = store.pool.majority_tier()
     res = _lib.residual(store.res_k)

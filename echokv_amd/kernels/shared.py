@@ -1,0 +1,164 @@
+"""Attention of a batch over a cached prefix that all of it shares, computed once.
+
+Sequences that begin with the same cached blocks (a system prompt, a document, the samples of
+one request) have the same keys there. ``prefix_attention`` reads and dequantizes those keys
+once for every query row of the batch; ``shared_prefix_decode`` is paged decode
+(``kernels.decode.decode_attention``) of such a batch: the shared blocks once, each sequence's
+own blocks as before, joined by log-sum-exp. The reference has no counterpart: its builder
+takes vLLM's ``common_prefix_len`` and does not use it (``echokv_vllm/backend.py:337-496``).
+
+The prefix is cut into ranges by the number of query rows, so a sequence's result depends on
+its batch through float rounding (``decode_attention`` alone is batch-invariant).
+
+Kernels: ``echokv_amd/csrc/attend_any.hip``, through ``echokv_prefix`` and
+``echokv_shared_decode``.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from echokv_amd import _lib
+from echokv_amd.kernels import decode as dec
+
+
+def _query(store, query: torch.Tensor) -> torch.Tensor:
+    L = store.layout
+    if query.dim() != 3 or query.shape[2] != L.head_size or query.shape[1] == 0 or query.shape[1] % L.num_kv_heads:
+        raise ValueError(f"query of shape {tuple(query.shape)} does not fit {L.num_kv_heads} KV heads of {L.head_size}")
+    return query if query.stride(2) == 1 else query.contiguous()
+
+
+def _blocks(store, blocks: torch.Tensor, prefix_len: int) -> torch.Tensor:
+    need = -(-prefix_len // store.layout.block_size)
+    if blocks.dim() != 1 or blocks.numel() < need:
+        raise ValueError(f"blocks must list the {need} blocks of a prefix of {prefix_len} tokens")
+    blocks = blocks[:need]
+    return blocks if blocks.dtype == torch.int32 and blocks.stride(0) == 1 else blocks.to(torch.int32).contiguous()
+
+
+def _workspace(workspace: torch.Tensor | None, need: int, device) -> torch.Tensor:
+    if workspace is None:
+        return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+    if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
+        raise ValueError(f"the workspace must be {need} contiguous uint8 bytes")
+    if workspace.data_ptr() % 16:
+        raise ValueError("the workspace must be aligned to 16 bytes")
+    return workspace
+
+
+def prefix_attention(store, query: torch.Tensor, blocks: torch.Tensor, prefix_len: int, softmax_scale: float,
+                     part: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of every row of ``query [T, Hq, D]`` over the first ``prefix_len`` cached tokens
+    of the block list ``blocks`` (int32 ``[>= ceil(prefix_len / block_size)]``), each read once.
+
+    Returns ``(part, lse)``: normalized float32 rows ``[T, Hq, D]`` and their log-sum-exp
+    ``[T, Hq]`` in log2 units (zeros and -inf for an empty prefix), what
+    ``kernels.prompt.prompt_attention`` takes as ``prefix``. ``workspace``: uint8,
+    ``prefix_workspace_bytes(...)``; by default the call allocates it."""
+    query = _query(store, query)
+    t, hq, d = query.shape
+    prefix_len = int(prefix_len)
+    need = prefix_workspace_bytes(store, hq, t, prefix_len)
+    _lib.require_current(query, blocks, part, lse, workspace, store.pages)
+    blocks = _blocks(store, blocks, prefix_len)
+    if part is None:
+        part = torch.empty(t, hq, d, device=query.device, dtype=torch.float32)
+    if part.dtype != torch.float32 or part.shape != query.shape or part.stride(2) != 1:
+        raise ValueError(f"part must be float32 {tuple(query.shape)} with contiguous channels")
+    if lse is None:
+        lse = torch.empty(t, hq, device=query.device, dtype=torch.float32)
+    if lse.dtype != torch.float32 or lse.shape != (t, hq) or not lse.is_contiguous():
+        raise ValueError(f"lse must be contiguous float32 {(t, hq)}")
+    ws = _workspace(workspace, need, query.device)
+    res = _lib.residual(store.res_k)
+    _lib.call(
+        "echokv_prefix", _lib.byref(store.abi), _lib.ptr(store.pages), _lib.ptr(store.block_res),
+        _lib.ptr(store.res_group), _lib.byref(res), _lib.ptr(query), query.stride(0), query.stride(1),
+        _lib.dtype_code(query), hq, None, t, _lib.ptr(blocks), prefix_len, float(softmax_scale), _lib.ptr(ws),
+        ws.numel(), _lib.ptr(part), part.stride(0), part.stride(1), _lib.ptr(lse), _lib.stream(),
+    )
+    return part, lse
+
+
+def prefix_workspace_bytes(store, num_q_heads: int, num_rows: int, prefix_len: int) -> int:
+    """Workspace of a ``prefix_attention`` call."""
+    return _lib.size("echokv_prefix_workspace", _lib.byref(store.abi), num_q_heads, num_rows, prefix_len)
+
+
+def shared_workspace_bytes(store, num_q_heads: int, num_seqs: int, prefix_len: int, num_splits: int) -> int:
+    """Workspace of a ``shared_prefix_decode`` call."""
+    return _lib.size("echokv_shared_decode_workspace", _lib.byref(store.abi), num_q_heads, num_seqs, prefix_len,
+                     num_splits)
+
+
+def suffix_splits(block_table: torch.Tensor, block_size: int, prefix_len: int, blocks_per_split: int,
+                  max_len: int | None) -> int:
+    """Splits of the tokens behind the prefix when the caller names none."""
+    cols = max(0, block_table.shape[1] - prefix_len // block_size)
+    longest = cols if max_len is None else min(cols, -(-max(0, max_len - prefix_len) // block_size))
+    return max(dec.SHORT_SPLITS, min(-(-longest // blocks_per_split), dec.MAX_SPLITS))
+
+
+def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                         prefix_len: int, softmax_scale: float, blocks_per_split: int = dec.BLOCKS_PER_SPLIT,
+                         q_rows: torch.Tensor | None = None, bt_rows: torch.Tensor | None = None,
+                         blocks: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                         max_len: int | None = None, num_splits: int | None = None,
+                         workspace: torch.Tensor | None = None, tier: int | None = None,
+                         tier_mask: torch.Tensor | str | None = None) -> torch.Tensor:
+    """``decode_attention`` of sequences whose first ``prefix_len`` tokens (a multiple of the
+    block size) are the same cached blocks, which are read once for the batch.
+
+    Arguments as ``decode_attention``'s; ``seq_lens[i]`` counts the prefix, and row
+    ``bt_rows[i]`` of the block table begins with the shared blocks. ``blocks``: their list (int32), by
+    default the first row of the table. A sequence shorter than ``prefix_len`` (length 0:
+    graph padding) leaves its row untouched. ``num_splits`` and ``max_len``'s default splits cut the
+    tokens behind the prefix. ``workspace``: uint8, ``shared_workspace_bytes(...)``; by default the
+    call allocates it. A prefix of 0 tokens is plain decode."""
+    prefix_len = int(prefix_len)
+    if prefix_len == 0:
+        return dec.decode_attention(store, query, block_table, seq_lens, softmax_scale, blocks_per_split, q_rows,
+                                    bt_rows, out, max_len, num_splits, None, tier, True, tier_mask)
+    L = store.layout
+    if prefix_len < 0 or prefix_len % L.block_size:
+        raise ValueError(f"prefix_len must be a multiple of the block size {L.block_size}, got {prefix_len}")
+    query = _query(store, query)
+    hq, d = query.shape[1:]
+    s = seq_lens.shape[0]
+    _lib.require_current(query, block_table, seq_lens, q_rows, bt_rows, blocks, out, workspace, store.pages)
+    if q_rows is None and query.shape[0] < s:
+        raise ValueError(f"{s} sequences, {query.shape[0]} query rows")
+    if block_table.dim() != 2 or block_table.shape[1] * L.block_size < prefix_len:
+        raise ValueError(f"the block table holds fewer than {prefix_len} tokens a row")
+    if block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        block_table = block_table.to(torch.int32).contiguous()
+    if s and blocks is None and block_table.shape[0] == 0:
+        raise ValueError("the block table has no row to take the shared blocks from")
+    if num_splits is None:
+        num_splits = suffix_splits(block_table, L.block_size, prefix_len, blocks_per_split, max_len)
+    need = shared_workspace_bytes(store, hq, s, prefix_len, int(num_splits))
+    dev = query.device
+    lens, q_rows, bt_rows = (dec._i64(t, dev) for t in (seq_lens, q_rows, bt_rows))
+    if out is None:
+        out = torch.empty(s if q_rows is None else query.shape[0], hq, d, device=dev, dtype=torch.float32)
+    if out.dim() != 3 or out.shape[1:] != query.shape[1:] or out.stride(2) != 1:
+        raise ValueError("out must be [rows, Hq, D] with contiguous channels")
+    if s == 0:
+        return out
+    blocks = _blocks(store, block_table[0] if blocks is None else blocks, prefix_len)
+    tier_mask = dec.tier_mask_of(store, tier_mask, dev)
+    if tier is None:
+        tier = store.pool.majority_tier()
+    ws = _workspace(workspace, need, dev)
+    res = _lib.residual(store.res_k)
+    _lib.call(
+        "echokv_shared_decode", _lib.byref(store.abi), _lib.ptr(store.pages), _lib.ptr(store.block_res),
+        _lib.ptr(store.res_group), _lib.byref(res), _lib.ptr(query), query.stride(0), query.stride(1),
+        _lib.dtype_code(query), hq, _lib.ptr(q_rows), _lib.ptr(block_table), block_table.stride(0), _lib.ptr(bt_rows),
+        _lib.ptr(lens), s, _lib.ptr(blocks), prefix_len, float(softmax_scale), int(num_splits), int(blocks_per_split),
+        int(tier), _lib.ptr(tier_mask), _lib.ptr(ws), ws.numel(), _lib.ptr(out), out.stride(0), out.stride(1),
+        _lib.dtype_code(out), _lib.stream(),
+    )
+    return out

@@ -277,6 +277,59 @@ int echokv_prefill_own_group(const echokv_layout* L, const uint8_t* pages, const
                              void* out, int64_t o_s0, int64_t o_s1, int32_t out_dtype,
                              float softmax_scale, echokv_stream_t stream);
 
+/* Causal attention of packed prompts over their own keys and values, all of one dtype:
+ * query [rows, num_q_heads, D], key and value [rows, num_kv_heads, D] (strides per row and
+ * head, contiguous channels; row t of a sequence sees its key rows up to t). tiles [n_tiles, 4]
+ * int32 = (the sequence's first row, its tokens, the tile's first token, its tokens <= tile_m),
+ * tile_m = echokv_prompt_tile_m(...); rows outside every tile are left as they are. part
+ * (nullable, float32 rows like the output's, strides p_s0 / p_s1) and part_lse (float
+ * [rows, num_q_heads], log2-domain log-sum-exp, -inf: none): attention of the same query rows over
+ * keys before the prompt (echokv_prefix's), joined with the result. lse (nullable, same shape)
+ * receives each row's log-sum-exp, the part's keys included. head_size a multiple of 4 up to
+ * 256. No counterpart in the reference, whose prefill reads the cache
+ * (echokv_vllm/kernels/prefill.py:170-207).
+ * echokv_prompt_tile_m: query tokens per tile, or minus an error code. */
+int32_t echokv_prompt_tile_m(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_size);
+int echokv_prompt(const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0, int64_t k_s1,
+                  const void* value, int64_t v_s0, int64_t v_s1, int32_t dtype, int32_t num_q_heads,
+                  int32_t num_kv_heads, int32_t head_size, const int32_t* tiles, int64_t n_tiles, int32_t tile_m,
+                  float softmax_scale, const float* part, int64_t p_s0, int64_t p_s1, const float* part_lse,
+                  void* out, int64_t o_s0, int64_t o_s1, int32_t out_dtype, float* lse, echokv_stream_t stream);
+
+/* Attention of n query rows (q_rows[i], NULL = i) over the same cached keys, each key read
+ * once for all of them: the first prefix_len tokens of the block list `blocks` (device int32,
+ * ceil(prefix_len / block_size) entries). part (float32, row q_rows[i], strides p_s0 / p_s1) gets
+ * the normalized rows and lse (float [rows, num_q_heads]) their log2-domain log-sum-exp (zeros
+ * and -inf for prefix_len 0). workspace: echokv_prefix_workspace(...) bytes, 16-byte aligned.
+ * Results depend on n through float rounding (the keys are cut into ranges by it).
+ * No counterpart in the reference. */
+int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t n, int64_t prefix_len);
+int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res, const int64_t* res_group,
+                  const echokv_residual* res, const void* query, int64_t q_s0, int64_t q_s1, int32_t q_dtype,
+                  int32_t num_q_heads, const int64_t* q_rows, int64_t n, const int32_t* blocks, int64_t prefix_len,
+                  float softmax_scale, void* workspace, int64_t workspace_bytes, float* part, int64_t p_s0,
+                  int64_t p_s1, float* lse, echokv_stream_t stream);
+
+/* Paged decode of a batch whose sequences begin with the same cached blocks: sequence i's
+ * block-table row starts with `blocks` (prefix_len tokens, a positive multiple of block_size);
+ * they are read once for the batch, each sequence's further seq_lens[i] - prefix_len tokens
+ * by the split schedule of echokv_decode (same q_rows, bt_rows, num_splits, blocks_per_split,
+ * tier and tier_mask; num_splits cuts the tokens behind the prefix), and both are joined into
+ * out[q_rows[i]]. Sequences shorter than prefix_len (length 0: graph padding) leave their row
+ * untouched. workspace: echokv_shared_decode_workspace(...) bytes, 16-byte aligned. Results
+ * depend on num_seqs through float rounding. No counterpart in the reference, whose builder
+ * leaves its common_prefix_len unused (echokv_vllm/backend.py:337-496). */
+int64_t echokv_shared_decode_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t num_seqs,
+                                       int64_t prefix_len, int32_t num_splits);
+int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,
+                         const int64_t* res_group, const echokv_residual* res, const void* query, int64_t q_s0,
+                         int64_t q_s1, int32_t q_dtype, int32_t num_q_heads, const int64_t* q_rows,
+                         const int32_t* block_table, int64_t bt_s0, const int64_t* bt_rows, const int64_t* seq_lens,
+                         int64_t num_seqs, const int32_t* blocks, int64_t prefix_len, float softmax_scale,
+                         int32_t num_splits, int32_t blocks_per_split, int32_t tier, const int32_t* tier_mask,
+                         void* workspace, int64_t workspace_bytes, void* out, int64_t o_s0, int64_t o_s1,
+                         int32_t out_dtype, echokv_stream_t stream);
+
 /* Dense dequantization of prefill contexts: work [n, 4] int32 = (block-table row,
  * block index, dense row of the block's first token, ctx) -> K, V [*, H, D].
  * Replaces echokv_vllm/kernels/prefill.py:90-115 (dequant_dense), kernel 330-369. */
