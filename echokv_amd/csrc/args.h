@@ -358,7 +358,9 @@ struct FlashArgs {
 
 // Causal attention of packed prompts over their own keys and values: query row t of a
 // sequence sees key rows [first row, t]. Rows of a tile are (token, GQA head) pairs.
-constexpr int kPromptRows = 256;     // query rows of a tile
+// Query rows of a tile: 32 per wave of the 16-bit kernel (head size 256: four waves, whose
+// accumulators take the registers of eight).
+inline int prompt_rows(int head_size) { return head_size > 128 ? 128 : 256; }
 struct PromptArgs {
   const void* q;
   long q_s0, q_s1;
@@ -482,6 +484,8 @@ size_t canary_lds_bytes(int d, int nbits, int kg);  // one canary workgroup's LD
 hipError_t launch_prefill(const PrefillArgs& a, long n, long n_merges, hipStream_t s);
 hipError_t launch_prefill_pack(const PackArgs& a, long n_packs, hipStream_t s);
 hipError_t launch_prefill_flash(const FlashArgs& a, hipStream_t s);
+bool prompt_mfma(const PromptArgs& a);  // whether the 16-bit kernel takes the call
+hipError_t launch_prompt(const PromptArgs& a, hipStream_t s);
 hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s);
 hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s);
 hipError_t launch_join(const JoinArgs& a, hipStream_t s);

@@ -1,0 +1,353 @@
+// Causal attention of packed prompts on 16-bit matrix instructions: float16 or bfloat16 rows of
+// head size 64, 128 or 256 (attend_any.hip takes every other case).
+//
+// One workgroup per (query tile, KV head): 32 query rows per wave, rows are (token, GQA head)
+// pairs of one KV head, so its heads share every key and value that is read. The tile's keys
+// stream in steps of 64 through a ring in LDS, keys and values row-major as they lie in memory
+// (direct global-to-LDS loads of 16 bytes a lane, rows past the sequence clamped to its last
+// one), and each wave runs S^T, an online softmax and O^T per step (tiles.h). Scores and sums are
+// float32; the weights are rounded to the inputs' type for the value product (half a step of it,
+// 2^-8 or 2^-11, relative to each weight), float16 ones times 2^6 so that small ones keep their
+// bits.
+//
+// A value that is infinite or NaN must not reach rows that do not see its key (their weight is
+// 0, and 0 x inf is NaN). Steps with a causal edge look for one; a wave that finds one computes
+// its rows again, with such values out of the products and added where they are seen.
+#include "tiles.h"
+
+namespace ek {
+namespace {
+
+constexpr int kKeys = 64;
+constexpr float kInf = __builtin_inff();
+
+template <int D, int WAVES>
+struct Ring {
+  static constexpr int SIDE = kKeys * D * 2;  // bytes of a step's keys, then its values
+  static constexpr int STEP = 2 * SIDE;
+  static constexpr int SLOTS = D == 256 ? 2 : 3;
+  static constexpr int NDMA = STEP / 1024 / WAVES;
+};
+
+}  // namespace
+
+template <int D, bool BF, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
+  using R = Ring<D, WAVES>;
+  constexpr int NS = D / 16, NDB = D / 32, NDMA = R::NDMA, SLOTS = R::SLOTS;
+  constexpr uint32_t kTop = BF ? 0x7f80u : 0x7c00u;  // infinity's bits
+  constexpr float kShift = BF ? 0.f : 6.f;  // float16 weights are 2^6 times the softmax's
+  extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int j = lane & 31, hh = lane >> 5;
+  const int h = (int)(blockIdx.x % a.H);  // heads fastest: with 8 of them an XCD's L2 holds one head's rows
+  const int32_t* td = a.tiles + 4 * (long)(blockIdx.x / a.H);
+  const long row0 = td[0];
+  const int seq = td[1], t0 = td[2], n_rows = td[3] * a.gqa;
+  const int kv_end = min(seq, t0 + td[3]);
+  const int n_steps = (kv_end + kKeys - 1) / kKeys;
+
+  const int r = 32 * wave + j;
+  const bool live = r < n_rows;
+  const bool active = 32 * wave < n_rows;
+  const int rc = live ? r : n_rows - 1;
+  const int pos = t0 + rc / a.gqa, qh = h * a.gqa + rc % a.gqa;
+  const int first_pos = t0 + 32 * wave / a.gqa;                              // the wave's first row's
+  const int last_pos = t0 + min(32 * wave + 31, n_rows - 1) / a.gqa;  // and last row's position
+
+  // This lane's share of a step's loads: byte offsets from the step's first key row. The
+  // permutation of LDS slots is made on the memory side, since LDS fills in lane order.
+  const uint32_t k_row = (uint32_t)a.k_s0 * 2, v_row = (uint32_t)a.v_s0 * 2;
+  const uint8_t* kbase = (const uint8_t*)a.k + 2 * (row0 * a.k_s0 + (long)h * a.k_s1);
+  const uint8_t* vbase = (const uint8_t*)a.v + 2 * (row0 * a.v_s0 + (long)h * a.v_s1);
+  const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
+  auto issue = [&](int step) {
+    const int kb = step * kKeys;
+    const uint8_t* kg = uniform_ptr(kbase + (long)kb * a.k_s0 * 2);
+    const uint8_t* vg = uniform_ptr(vbase + (long)kb * a.v_s0 * 2);
+    const uint32_t to = ring0 + (uint32_t)((step % SLOTS) * R::STEP + 1024 * NDMA * wave);
+    const int last = kv_end - 1 - kb;
+#pragma unroll
+    for (int i = 0; i < NDMA; ++i) {
+      const int p = 1024 * (NDMA * wave + i);
+      const bool val = p >= R::SIDE;  // wave-uniform
+      const int q = (p & (R::SIDE - 1)) + 16 * lane;
+      const int key = q / (2 * D), slot = q % (2 * D) / 16;
+      const int row = min(key, last);
+      const uint32_t off = (uint32_t)row * (val ? v_row : k_row) + 16 * (slot ^ (val ? v_swz<D>(key) : k_swz<D>(key)));
+      dma16(val ? vg : kg, off, to + 1024 * i);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS - 1; ++i)
+    if (i < n_steps) issue(i);
+
+  // Query fragments (B operand): row r, channels 16 s + 8 hh .. + 8. Scores are scaled inside
+  // the exponent and their maximum is taken before, which needs the scale positive: a negative
+  // one flips the query's sign, a zero one becomes 2^-100.
+  constexpr float kTiny = 7.8886090522101181e-31f;
+  const float scale = fabsf(a.scale_log2) < kTiny ? kTiny : fabsf(a.scale_log2);  // NaN stays
+  h8_t q[NS];
+  {
+    const uint16_t* src = (const uint16_t*)a.q + (row0 + pos) * a.q_s0 + (long)qh * a.q_s1 + 8 * hh;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) q[s] = *(const h8_t*)(src + 16 * s);
+    if (a.scale_log2 < 0.f) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        u4_t w = __builtin_bit_cast(u4_t, q[s]);
+        w ^= 0x80008000u;
+        q[s] = __builtin_bit_cast(h8_t, w);
+      }
+    }
+  }
+
+  f16v_t acc[NDB];
+  float m_run, lsum;
+  auto clear = [&]() {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) acc[db] = f16v_t{};
+    m_run = -kInf;
+    lsum = 0.f;
+  };
+  // Scores of the step at key kb0 to rounded weights (p[ks]: 16 keys), online. `edge`: some row
+  // does not see the whole step.
+  auto softmax = [&](f16v_t* s, int kb0, bool edge, u4_t* p) {
+    float mx = -kInf;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = kb0 + 32 * kb + 8 * (i >> 2) + 4 * hh + (i & 3);
+        s[kb][i] = edge && key > pos ? -kInf : s[kb][i];
+        mx = fmaxf(mx, s[kb][i]);
+      }
+    const float mt = halves_max(mx) * scale;
+    // The running maximum moves only when a row's passes it by more than 2^8: weights stay
+    // below 2^8 meanwhile.
+    if (__builtin_amdgcn_ballot_w64(mt > m_run + 8.f)) {
+      const float m_new = fmaxf(m_run, mt);
+      const float alpha = m_new == -kInf ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+      lsum *= alpha;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
+      m_run = m_new;
+    }
+    const float ms = m_run == -kInf ? 0.f : m_run - kShift;
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], scale, -ms));
+        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], scale, -ms));
+        sum[0] += x;
+        sum[1] += y;
+        p[2 * kb + (i >> 3)][(i & 7) >> 1] = pack2<BF>(x, y);
+      }
+    lsum += sum[0] + sum[1];
+  };
+
+  clear();
+  bool odd = false;  // a step with an edge holds an infinite value or NaN
+  for (int step = 0; step < n_steps; ++step) {
+    // Step `step` has landed once at most the loads of the steps after it remain.
+    if (SLOTS == 3 && step + 1 < n_steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NDMA) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (step + SLOTS - 1 < n_steps) issue(step + SLOTS - 1);
+    const int kb0 = step * kKeys;
+    if (!active || odd || kb0 > last_pos) continue;
+    const uint8_t* kt = ring + (step % SLOTS) * R::STEP;
+    const uint8_t* vt = kt + R::SIDE;
+
+    // Fragments two contraction steps at a time, the next ones requested before the products of
+    // the current (scheduling fences keep that order, and their registers).
+    f16v_t s[2] = {f16v_t{}, f16v_t{}};
+    {
+      h8_t f[2][4];
+      auto load = [&](int g, h8_t* x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = k_frag<D>(kt, i & 1, 2 * g + (i >> 1), j, hh);
+      };
+      load(0, f[0]);
+#pragma unroll
+      for (int g = 0; g < NS / 2; ++g) {
+        if (g + 1 < NS / 2) load(g + 1, f[(g + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i & 1] = mma<BF>(f[g & 1][i], q[2 * g + (i >> 1)], s[i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    const bool edge = kb0 + kKeys > first_pos + 1;
+    if (edge) {
+      typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+      us2_t m = {0, 0};
+#pragma unroll 4
+      for (int i = 0; i < R::SIDE / 1024; ++i) {
+        const u4_t w = *(const u4_t*)(vt + 1024 * i + 16 * lane);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2_t, w[e] & 0x7fff7fffu));
+      }
+      odd = __builtin_amdgcn_ballot_w64(m[0] >= kTop || m[1] >= kTop);
+    }
+    u4_t p[4];
+    softmax(s, kb0, edge, p);
+    {
+      constexpr int NG = NDB < 4 ? NDB : 4, NP = NDB / NG;  // channel blocks of a group, groups of 16 keys
+      h8_t f[2][NG];
+      auto load = [&](int g, h8_t* x) {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) x[i] = v_frag<D>(vt, g / NP, g % NP * NG + i, lane);
+      };
+      load(0, f[0]);
+#pragma unroll
+      for (int g = 0; g < 4 * NP; ++g) {
+        if (g + 1 < 4 * NP) load(g + 1, f[(g + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          const int db = g % NP * NG + i;
+          acc[db] = mma<BF>(f[g & 1][i], __builtin_bit_cast(h8_t, p[g / NP]), acc[db]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  // Rare: the wave's rows once more, from memory. The products leave infinite values and NaN out;
+  // which of them a row sees is a product of its own, of 0 / 1 weights with 1 for +inf, 2^7 for
+  // -inf and 2^14 for NaN (at most 64 of each a step: the sum tells them apart).
+  if (odd) {
+    clear();
+#pragma unroll 1
+    for (int kb0 = 0; kb0 <= last_pos; kb0 += kKeys) {
+      f16v_t s[2] = {f16v_t{}, f16v_t{}};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const uint8_t* row = kbase + 2 * (long)min(kb0 + 32 * kb + j, kv_end - 1) * a.k_s0 + 16 * hh;
+#pragma unroll
+        for (int c = 0; c < NS; ++c) s[kb] = mma<BF>(*(const h8_t*)(row + 32 * c), q[c], s[kb]);
+      }
+      u4_t p[4];
+      softmax(s, kb0, true, p);
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        uint32_t seen[4];
+        const uint16_t* row[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = kb0 + 16 * ks + 8 * (e >> 2) + 4 * hh + (e & 3);
+          row[e] = (const uint16_t*)(vbase + 2 * (long)min(key, kv_end - 1) * a.v_s0) + j;
+          if (!(e & 1)) seen[e >> 1] = pack2<BF>(key <= pos ? 1.f : 0.f, key + 1 <= pos ? 1.f : 0.f);
+        }
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          u4_t w, kinds;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t x[2], k[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              x[u] = row[2 * e + u][32 * db];
+              const bool bad = (x[u] & 0x7fffu) >= kTop;
+              k[u] = pack2<BF>((x[u] & 0x7fffu) > kTop ? 16384.f : x[u] & 0x8000u ? 128.f : 1.f, 0.f);
+              k[u] = bad ? k[u] : 0;
+              x[u] = bad ? 0 : x[u];
+            }
+            w[e] = x[0] | x[1] << 16;
+            kinds[e] = k[0] | k[1] << 16;
+          }
+          acc[db] = mma<BF>(__builtin_bit_cast(h8_t, w), __builtin_bit_cast(h8_t, p[ks]), acc[db]);
+          f16v_t found = f16v_t{};
+          found = mma<BF>(__builtin_bit_cast(h8_t, kinds), __builtin_bit_cast(h8_t, u4_t{seen[0], seen[1], seen[2], seen[3]}),
+                          found);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int n = (int)found[i];
+            float x = n & 127 ? kInf : 0.f;
+            x = n >> 7 & 127 ? (n & 127 ? __builtin_nanf("") : -kInf) : x;
+            acc[db][i] += n >> 14 ? __builtin_nanf("") : x;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  }
+
+  const float l = halves_sum(lsum);
+  if (!live) return;
+  const long row = row0 + pos, lr = row * a.hq + qh;
+  float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -kInf : m_run - kShift + __log2f(l), wp = 0.f;
+  if (a.part) {
+    const float pl = a.part_lse[lr], mx = fmaxf(pl, lse);
+    if (mx != -kInf) {
+      const float ep = __builtin_amdgcn_exp2f(pl - mx), eo = __builtin_amdgcn_exp2f(lse - mx), sum = ep + eo;
+      wp = ep / sum;
+      inv *= eo / sum;
+      lse = mx + __log2f(sum);
+    }
+  }
+  if (a.lse && hh == 0) a.lse[lr] = lse;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) acc[db] *= inv;
+  if (wp != 0.f) {
+    const float* src = a.part + row * a.p_s0 + (long)qh * a.p_s1 + 4 * hh;
+    typedef float f4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f4_t x = *(const f4_any_t*)(src + 32 * db + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[db][4 * g + e] = __builtin_fmaf(wp, x[e], acc[db][4 * g + e]);
+      }
+  }
+  const long ob = row * a.o_s0 + (long)qh * a.o_s1 + 4 * hh;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = acc[db][4 * g + e];
+      st_n<4>(a.out, a.out_dtype, ob + 32 * db + 8 * g, y);
+    }
+}
+
+bool prompt_mfma(const PromptArgs& a) {
+  if (a.dtype == ECHOKV_F32 || (a.D != 64 && a.D != 128 && a.D != 256)) return false;
+  // Rows aligned for 16-byte loads; a step's rows within 31 bits of bytes.
+  auto rows_ok = [](const void* p, long s0, long s1) {
+    return (uintptr_t)p % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s0 >= 0 && s0 < (1L << 30) / kKeys;
+  };
+  return a.gqa <= prompt_rows(a.D) && rows_ok(a.q, 0, 0) && a.q_s0 % 8 == 0 && a.q_s1 % 8 == 0 && rows_ok(a.k, a.k_s0, a.k_s1) &&
+         rows_ok(a.v, a.v_s0, a.v_s1);
+}
+
+template <int D, bool BF, int WAVES>
+static hipError_t launch_t(const PromptArgs& a, hipStream_t s) {
+  using R = Ring<D, WAVES>;
+  constexpr int lds = R::SLOTS * R::STEP;
+  static std::atomic<uint64_t> attr_done{0};
+  const hipError_t e = ensure_lds_limit((const void*)prompt_kernel<D, BF, WAVES>, lds, &attr_done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((prompt_kernel<D, BF, WAVES>), dim3((unsigned)((long)a.n_tiles * a.H)), dim3(64 * WAVES), lds, s, a);
+  return hipGetLastError();
+}
+
+template <int D, int WAVES>
+static hipError_t launch_d(const PromptArgs& a, hipStream_t s) {
+  return a.dtype == ECHOKV_BF16 ? launch_t<D, true, WAVES>(a, s) : launch_t<D, false, WAVES>(a, s);
+}
+
+hipError_t launch_prompt(const PromptArgs& a, hipStream_t s) {
+  if (a.D == 64) return launch_d<64, 8>(a, s);
+  if (a.D == 128) return launch_d<128, 8>(a, s);
+  if (a.D == 256) return launch_d<256, 4>(a, s);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace ek

@@ -1,0 +1,101 @@
+// 64-key steps of the 16-bit attention kernels (prompt.hip, shared.hip): keys and values
+// row-major in LDS as 16-bit elements, products by v_mfma_f32_32x32x16 with a wave's 32 query
+// rows as columns:
+//   S^T[key, row] = K Q^T,   O^T[d, row] += V^T P^T.
+// Lane (j = lane % 32, hh = lane / 32) holds column j. Register i of a 32-key S^T accumulator is
+// key 8 (i / 4) + 4 hh + i % 4, so registers 8 u .. 8 u + 7 are the lane's share of a 16-key
+// contraction of O^T: no exchange, as long as V^T's operand lists the keys in that order. It is
+// read from the row-major values by the transposing LDS read (ds_read_b64_tr_b16): of 16
+// lanes, lane a addresses four channels 4 (a % 4) of row a / 4, and lane i receives channel i of
+// the four rows.
+#pragma once
+
+#include "args.h"
+
+namespace ek {
+
+typedef float f16v_t __attribute__((ext_vector_type(16)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+// Fragments are kept as bits: h8_t whatever the type.
+template <bool BF>
+__device__ __forceinline__ f16v_t mma(const h8_t a, const h8_t b, const f16v_t c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Two floats rounded to the 16-bit type, as bits.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  if constexpr (BF) {
+    typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, b2_t{(__bf16)x, (__bf16)y});
+  } else {
+    return __builtin_bit_cast(uint32_t, h2_t{(_Float16)x, (_Float16)y});
+  }
+}
+
+// LDS rows are unpadded; 16-byte slots are permuted by row. K: 32 rows are read at one slot of
+// each. V: the transposing read takes four neighbouring rows at 32 bytes of each, next to
+// another 16 lanes at the next 32 bytes.
+template <int D>
+__device__ __forceinline__ int k_swz(int key) {
+  return D == 64 ? (key >> 1) & 7 : key & 15;
+}
+template <int D>
+__device__ __forceinline__ int v_swz(int key) {
+  return D == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3);
+}
+
+// max / sum of x over the two half-waves (lanes l and l ^ 32).
+__device__ __forceinline__ float halves_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float halves_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
+  const uint64_t u = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return (const uint8_t*)(((uint64_t)hi << 32) | lo);
+}
+
+// 16 bytes per lane from base + off to LDS [lds, lds + 1024) in lane order.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, %2" ::"v"(off), "s"(__builtin_amdgcn_readfirstlane(lds)),
+               "s"(base)
+               : "memory", "m0");
+}
+
+// K fragment (A operand of S^T): key rows 32 kb + j, channels 16 s + 8 hh .. + 8.
+template <int D>
+__device__ __forceinline__ h8_t k_frag(const uint8_t* k, int kb, int s, int j, int hh) {
+  const int key = 32 * kb + j;
+  return *(const h8_t*)(k + key * (2 * D) + 16 * ((2 * s + hh) ^ k_swz<D>(key)));
+}
+
+// V^T fragment (A operand of O^T): channels 32 db + j, keys 16 ks + {4 hh .. + 3, 8 + 4 hh .. + 3}.
+template <int D>
+__device__ __forceinline__ h8_t v_frag(const uint8_t* v, int ks, int db, int lane) {
+  const int a = lane & 15, hh = lane >> 5, g = (lane >> 4) & 1;
+  typedef __attribute__((address_space(3))) s4_t lds_s4;
+  s4_t x[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int key = 16 * ks + 8 * u + 4 * hh + (a >> 2);
+    const int slot = 4 * db + 2 * g + ((a & 3) >> 1);
+    const uint8_t* p = v + key * (2 * D) + 16 * (slot ^ v_swz<D>(key)) + 8 * (a & 1);
+    x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uint32_t)(uintptr_t)p);
+  }
+  return __builtin_bit_cast(h8_t, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+}  // namespace ek
