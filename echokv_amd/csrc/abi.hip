@@ -600,7 +600,7 @@ int echokv_prefill_own_group(const echokv_layout* L, const uint8_t* pages, const
 int32_t echokv_prompt_tile_m(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_size) {
   if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return -ECHOKV_ESHAPE;
   if (head_size <= 0 || head_size % 4 || head_size > ek::kMaxAnyD) return -ECHOKV_ESHAPE;
-  const int rows = ek::prompt_rows(head_size) / (num_q_heads / num_kv_heads);
+  const int rows = ek::kPromptRows / (num_q_heads / num_kv_heads);
   return rows < 1 ? 1 : rows;
 }
 

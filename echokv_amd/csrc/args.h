@@ -358,9 +358,7 @@ struct FlashArgs {
 
 // Causal attention of packed prompts over their own keys and values: query row t of a
 // sequence sees key rows [first row, t]. Rows of a tile are (token, GQA head) pairs.
-// Query rows of a tile: 32 per wave of the 16-bit kernel (head size 256: four waves, whose
-// accumulators take the registers of eight).
-inline int prompt_rows(int head_size) { return head_size > 128 ? 128 : 256; }
+constexpr int kPromptRows = 128;  // query rows of a tile: 32 for each of the 16-bit kernel's four waves
 struct PromptArgs {
   const void* q;
   long q_s0, q_s1;

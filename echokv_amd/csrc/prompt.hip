@@ -19,22 +19,23 @@ namespace ek {
 namespace {
 
 constexpr int kKeys = 64;
+constexpr int kWaves = 4;
+constexpr int kSlots = 2;  // steps in LDS: two workgroups fit a CU up to head size 128
 constexpr float kInf = __builtin_inff();
 
-template <int D, int WAVES>
+template <int D>
 struct Ring {
   static constexpr int SIDE = kKeys * D * 2;  // bytes of a step's keys, then its values
   static constexpr int STEP = 2 * SIDE;
-  static constexpr int SLOTS = D == 256 ? 2 : 3;
-  static constexpr int NDMA = STEP / 1024 / WAVES;
+    static constexpr int NDMA = STEP / 1024 / kWaves;
 };
 
 }  // namespace
 
-template <int D, bool BF, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
-  using R = Ring<D, WAVES>;
-  constexpr int NS = D / 16, NDB = D / 32, NDMA = R::NDMA, SLOTS = R::SLOTS;
+template <int D, bool BF>
+__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(PromptArgs a) {
+  using R = Ring<D>;
+  constexpr int NS = D / 16, NDB = D / 32, NDMA = R::NDMA;
   constexpr uint32_t kTop = BF ? 0x7f80u : 0x7c00u;  // infinity's bits
   constexpr float kShift = BF ? 0.f : 6.f;  // float16 weights are 2^6 times the softmax's
   extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
@@ -66,7 +67,7 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
     const int kb = step * kKeys;
     const uint8_t* kg = uniform_ptr(kbase + (long)kb * a.k_s0 * 2);
     const uint8_t* vg = uniform_ptr(vbase + (long)kb * a.v_s0 * 2);
-    const uint32_t to = ring0 + (uint32_t)((step % SLOTS) * R::STEP + 1024 * NDMA * wave);
+    const uint32_t to = ring0 + (uint32_t)((step % kSlots) * R::STEP + 1024 * NDMA * wave);
     const int last = kv_end - 1 - kb;
 #pragma unroll
     for (int i = 0; i < NDMA; ++i) {
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
     }
   };
 #pragma unroll
-  for (int i = 0; i < SLOTS - 1; ++i)
+  for (int i = 0; i < kSlots - 1; ++i)
     if (i < n_steps) issue(i);
 
   // Query fragments (B operand): row r, channels 16 s + 8 hh .. + 8. Scores are scaled inside
@@ -114,15 +115,18 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
   // Scores of the step at key kb0 to rounded weights (p[ks]: 16 keys), online. `edge`: some row
   // does not see the whole step.
   auto softmax = [&](f16v_t* s, int kb0, bool edge, u4_t* p) {
+    if (edge) {
+      const int left = pos - kb0 - 4 * hh;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) > left ? -kInf : s[kb][i];
+    }
     float mx = -kInf;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = kb0 + 32 * kb + 8 * (i >> 2) + 4 * hh + (i & 3);
-        s[kb][i] = edge && key > pos ? -kInf : s[kb][i];
-        mx = fmaxf(mx, s[kb][i]);
-      }
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
     const float mt = halves_max(mx) * scale;
     // The running maximum moves only when a row's passes it by more than 2^8: weights stay
     // below 2^8 meanwhile.
@@ -149,18 +153,22 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
     lsum += sum[0] + sum[1];
   };
 
+  uint32_t k_lane[NS], v_lane[NDB];
+#pragma unroll
+  for (int c = 0; c < NS; ++c) k_lane[c] = k_at<D>(c, j, hh);
+#pragma unroll
+  for (int db = 0; db < NDB; ++db) v_lane[db] = v_at<D>(db, lane);
   clear();
   bool odd = false;  // a step with an edge holds an infinite value or NaN
   for (int step = 0; step < n_steps; ++step) {
-    // Step `step` has landed once at most the loads of the steps after it remain.
-    if (SLOTS == 3 && step + 1 < n_steps) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NDMA) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // This wave's share of the step has landed, with the barrier every wave's; its loads were made a
+    // step ago, and the next step's go to the slot that every wave has left.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (step + SLOTS - 1 < n_steps) issue(step + SLOTS - 1);
+    if (step + kSlots - 1 < n_steps) issue(step + kSlots - 1);
     const int kb0 = step * kKeys;
     if (!active || odd || kb0 > last_pos) continue;
-    const uint8_t* kt = ring + (step % SLOTS) * R::STEP;
-    const uint8_t* vt = kt + R::SIDE;
+    const uint32_t kt = ring0 + (uint32_t)((step % kSlots) * R::STEP);
 
     // Fragments two contraction steps at a time, the next ones requested before the products of
     // the current (scheduling fences keep that order, and their registers).
@@ -169,7 +177,7 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
       h8_t f[2][4];
       auto load = [&](int g, h8_t* x) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = k_frag<D>(kt, i & 1, 2 * g + (i >> 1), j, hh);
+        for (int i = 0; i < 4; ++i) x[i] = k_read<D>(k_lane[2 * g + (i >> 1)] + kt, i & 1);
       };
       load(0, f[0]);
 #pragma unroll
@@ -187,7 +195,7 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
       us2_t m = {0, 0};
 #pragma unroll 4
       for (int i = 0; i < R::SIDE / 1024; ++i) {
-        const u4_t w = *(const u4_t*)(vt + 1024 * i + 16 * lane);
+        const u4_t w = *(const lds_t<u4_t>*)(kt + R::SIDE + 1024 * i + 16 * lane);
 #pragma unroll
         for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2_t, w[e] & 0x7fff7fffu));
       }
@@ -200,7 +208,7 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
       h8_t f[2][NG];
       auto load = [&](int g, h8_t* x) {
 #pragma unroll
-        for (int i = 0; i < NG; ++i) x[i] = v_frag<D>(vt, g / NP, g % NP * NG + i, lane);
+        for (int i = 0; i < NG; ++i) x[i] = v_read<D>(v_lane[g % NP * NG + i] + kt + R::SIDE, g / NP);
       };
       load(0, f[0]);
 #pragma unroll
@@ -295,7 +303,6 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
   for (int db = 0; db < NDB; ++db) acc[db] *= inv;
   if (wp != 0.f) {
     const float* src = a.part + row * a.p_s0 + (long)qh * a.p_s1 + 4 * hh;
-    typedef float f4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -305,16 +312,19 @@ __global__ __launch_bounds__(64 * WAVES) void prompt_kernel(PromptArgs a) {
         for (int e = 0; e < 4; ++e) acc[db][4 * g + e] = __builtin_fmaf(wp, x[e], acc[db][4 * g + e]);
       }
   }
-  const long ob = row * a.o_s0 + (long)qh * a.o_s1 + 4 * hh;
+  const long ob = row * a.o_s0 + (long)qh * a.o_s1;
+  if (a.out_dtype == ECHOKV_F32) {
+    float* dst = (float*)a.out + ob + 4 * hh;
 #pragma unroll
-  for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = acc[db][4 * g + e];
-      st_n<4>(a.out, a.out_dtype, ob + 32 * db + 8 * g, y);
-    }
+      for (int g = 0; g < 4; ++g)
+        *(f4_any_t*)(dst + 32 * db + 8 * g) = f4_t{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+  } else if (a.out_dtype == ECHOKV_BF16) {
+    store16<NDB, true>((uint8_t*)a.out + 2 * ob, acc, hh);
+  } else {
+    store16<NDB, false>((uint8_t*)a.out + 2 * ob, acc, hh);
+  }
 }
 
 bool prompt_mfma(const PromptArgs& a) {
@@ -323,30 +333,30 @@ bool prompt_mfma(const PromptArgs& a) {
   auto rows_ok = [](const void* p, long s0, long s1) {
     return (uintptr_t)p % 16 == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s0 >= 0 && s0 < (1L << 30) / kKeys;
   };
-  return a.gqa <= prompt_rows(a.D) && rows_ok(a.q, 0, 0) && a.q_s0 % 8 == 0 && a.q_s1 % 8 == 0 && rows_ok(a.k, a.k_s0, a.k_s1) &&
+  return a.gqa <= kPromptRows && rows_ok(a.q, 0, 0) && a.q_s0 % 8 == 0 && a.q_s1 % 8 == 0 && rows_ok(a.k, a.k_s0, a.k_s1) &&
          rows_ok(a.v, a.v_s0, a.v_s1);
 }
 
-template <int D, bool BF, int WAVES>
+template <int D, bool BF>
 static hipError_t launch_t(const PromptArgs& a, hipStream_t s) {
-  using R = Ring<D, WAVES>;
-  constexpr int lds = R::SLOTS * R::STEP;
+  using R = Ring<D>;
+  constexpr int lds = kSlots * R::STEP;
   static std::atomic<uint64_t> attr_done{0};
-  const hipError_t e = ensure_lds_limit((const void*)prompt_kernel<D, BF, WAVES>, lds, &attr_done);
+  const hipError_t e = ensure_lds_limit((const void*)prompt_kernel<D, BF>, lds, &attr_done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((prompt_kernel<D, BF, WAVES>), dim3((unsigned)((long)a.n_tiles * a.H)), dim3(64 * WAVES), lds, s, a);
+  hipLaunchKernelGGL((prompt_kernel<D, BF>), dim3((unsigned)((long)a.n_tiles * a.H)), dim3(64 * kWaves), lds, s, a);
   return hipGetLastError();
 }
 
-template <int D, int WAVES>
+template <int D>
 static hipError_t launch_d(const PromptArgs& a, hipStream_t s) {
-  return a.dtype == ECHOKV_BF16 ? launch_t<D, true, WAVES>(a, s) : launch_t<D, false, WAVES>(a, s);
+  return a.dtype == ECHOKV_BF16 ? launch_t<D, true>(a, s) : launch_t<D, false>(a, s);
 }
 
 hipError_t launch_prompt(const PromptArgs& a, hipStream_t s) {
-  if (a.D == 64) return launch_d<64, 8>(a, s);
-  if (a.D == 128) return launch_d<128, 8>(a, s);
-  if (a.D == 256) return launch_d<256, 4>(a, s);
+  if (a.D == 64) return launch_d<64>(a, s);
+  if (a.D == 128) return launch_d<128>(a, s);
+  if (a.D == 256) return launch_d<256>(a, s);
   return hipErrorInvalidValue;
 }
 

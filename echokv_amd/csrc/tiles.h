@@ -75,27 +75,59 @@ __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_
                : "memory", "m0");
 }
 
-// K fragment (A operand of S^T): key rows 32 kb + j, channels 16 s + 8 hh .. + 8.
+template <class T>
+using lds_t = __attribute__((address_space(3))) T;
+
+// K fragment (A operand of S^T): key rows 32 kb + j, channels 16 s + 8 hh .. + 8. k_at: the
+// lane's byte offset in the step's keys, k_read: the fragment at an LDS address made of it.
 template <int D>
-__device__ __forceinline__ h8_t k_frag(const uint8_t* k, int kb, int s, int j, int hh) {
-  const int key = 32 * kb + j;
-  return *(const h8_t*)(k + key * (2 * D) + 16 * ((2 * s + hh) ^ k_swz<D>(key)));
+__device__ __forceinline__ uint32_t k_at(int s, int j, int hh) {
+  return (uint32_t)(j * (2 * D) + 16 * ((2 * s + hh) ^ k_swz<D>(j)));  // k_swz has period 32
+}
+template <int D>
+__device__ __forceinline__ h8_t k_read(uint32_t at, int kb) {
+  return *(const lds_t<h8_t>*)(at + kb * 64 * D);
 }
 
 // V^T fragment (A operand of O^T): channels 32 db + j, keys 16 ks + {4 hh .. + 3, 8 + 4 hh .. + 3}.
 template <int D>
-__device__ __forceinline__ h8_t v_frag(const uint8_t* v, int ks, int db, int lane) {
+__device__ __forceinline__ uint32_t v_at(int db, int lane) {
   const int a = lane & 15, hh = lane >> 5, g = (lane >> 4) & 1;
-  typedef __attribute__((address_space(3))) s4_t lds_s4;
+  const int key = 4 * hh + (a >> 2), slot = 4 * db + 2 * g + ((a & 3) >> 1);  // v_swz has period 4
+  return (uint32_t)(key * (2 * D) + 16 * (slot ^ v_swz<D>(key)) + 8 * (a & 1));
+}
+template <int D>
+__device__ __forceinline__ h8_t v_read(uint32_t at, int ks) {
   s4_t x[2];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int key = 16 * ks + 8 * u + 4 * hh + (a >> 2);
-    const int slot = 4 * db + 2 * g + ((a & 3) >> 1);
-    const uint8_t* p = v + key * (2 * D) + 16 * (slot ^ v_swz<D>(key)) + 8 * (a & 1);
-    x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(uint32_t)(uintptr_t)p);
-  }
+  for (int u = 0; u < 2; ++u)
+    x[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t<s4_t>*)(at + (16 * ks + 8 * u) * 2 * D));
   return __builtin_bit_cast(h8_t, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+typedef float f4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// A lane's O^T column as a 16-bit row at `row` (any element alignment): the half-waves exchange
+// their channels of two groups of eight, so that each lane stores 16 consecutive bytes. Both
+// lanes of a column take part.
+template <int NDB, bool BF>
+__device__ __forceinline__ void store16(uint8_t* row, const f16v_t* acc, int hh) {
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      u4_any_t o;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t x = pack2<BF>(acc[db][4 * g + 2 * e], acc[db][4 * g + 2 * e + 1]);
+        const uint32_t y = pack2<BF>(acc[db][4 * g + 4 + 2 * e], acc[db][4 * g + 5 + 2 * e]);
+        const auto z = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+        o[e] = z[0];
+        o[2 + e] = z[1];
+      }
+      *(u4_any_t*)(row + 64 * db + 16 * g + 16 * hh) = o;
+    }
 }
 
 }  // namespace ek

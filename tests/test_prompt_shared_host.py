@@ -75,7 +75,7 @@ def test_prompt_refuses_shapes_and_types(lib):
 
 def _prompt(lib, **kw):
     p = C.c_void_p(64)  # never dereferenced: every call below fails its checks first
-    a = dict(dtype=_lib.BF16, hq=32, h=8, d=128, tiles=p, n=1, tile_m=64, part=None, part_lse=None, out=p, od=_lib.F16)
+    a = dict(dtype=_lib.BF16, hq=32, h=8, d=128, tiles=p, n=1, tile_m=32, part=None, part_lse=None, out=p, od=_lib.F16)
     a.update(kw)
     return lib.echokv_prompt(p, 4096, 128, p, 1024, 128, p, 1024, 128, a["dtype"], a["hq"], a["h"], a["d"], a["tiles"],
                              a["n"], a["tile_m"], 0.1, a["part"], 4096, 128, a["part_lse"], a["out"], 4096, 128, a["od"],
@@ -83,10 +83,10 @@ def _prompt(lib, **kw):
 
 
 def test_prompt_entry_rejects_bad_arguments(lib):
-    assert lib.echokv_prompt_tile_m(32, 8, 128) == 64
+    assert lib.echokv_prompt_tile_m(32, 8, 128) == 32
     for bad in ((30, 8, 128), (32, 0, 128), (32, 8, 260), (32, 8, 30)):
         assert lib.echokv_prompt_tile_m(*bad) == -2
-    for kw, code in ((dict(hq=30), 2), (dict(d=512), 2), (dict(tile_m=32), 2), (dict(dtype=7), 3), (dict(od=-1), 3),
+    for kw, code in ((dict(hq=30), 2), (dict(d=512), 2), (dict(tile_m=64), 2), (dict(dtype=7), 3), (dict(od=-1), 3),
                      (dict(n=-1), 1), (dict(n=1 << 40), 1), (dict(tiles=None), 1), (dict(out=None), 1),
                      (dict(part=C.c_void_p(64)), 1), (dict(n=0), 0)):
         assert _prompt(lib, **kw) == code, kw
