@@ -652,10 +652,19 @@ int echokv_prompt(const void* query, int64_t q_s0, int64_t q_s1, const void* key
 
 namespace {
 
+// Layouts of the 16-bit kernel: its items (4 keys x 8 channels) sit in one K group and V group.
+bool prefix_mfma(const echokv_layout* L) {
+  const int D = L->head_size;
+  return (D == 64 || D == 128 || D == 256) && !(L->block_size & (L->block_size - 1)) &&
+         !(L->k_group & (L->k_group - 1)) && L->k_group >= 4 && L->v_group % 8 == 0 && L->chunks_per_page <= 4 &&
+         L->num_blocks * L->chunks_per_page < (1LL << 24);
+}
+
 // Ranges of a shared prefix: enough workgroups for the chip (two for each of its 256
 // CUs) with at least 128 keys each.
 int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
-  const int64_t gqa = hq / L->num_kv_heads, wgs = (n * gqa + 63) / 64 * L->num_kv_heads;
+  const int64_t gqa = hq / L->num_kv_heads, rows = prefix_mfma(L) ? ek::kPrefixRows : 64;
+  const int64_t wgs = (n * gqa + rows - 1) / rows * L->num_kv_heads;
   int64_t r = (512 + wgs - 1) / wgs;
   const int64_t most = len / 128;
   r = r < most ? r : most;
@@ -694,7 +703,7 @@ ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const i
   a.len = (int)len;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.ranges = ranges;
-  a.per = (int)((len + ranges - 1) / ranges + 63) / 64 * 64;
+  a.per = (int)((len + ranges - 1) / ranges + 127) / 128 * 128;
   a.acc = (float*)workspace;
   a.ml = a.acc + ranges * n * hq * L->head_size;
   a.part = nullptr;
@@ -702,7 +711,15 @@ ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const i
   a.lse = nullptr;
   a.lens = nullptr;
   a.suffix = nullptr;
+  a.bs_shift = __builtin_ctz((unsigned)L->block_size);
+  a.kg_shift = __builtin_ctz((unsigned)L->k_group);
+  a.kc_mul = chunk_mul(L->chunks_per_page);
   return a;
+}
+
+hipError_t run_prefix(const echokv_layout* L, const ek::PrefixArgs& a, hipStream_t s) {
+  const bool mfma = prefix_mfma(L) && (uintptr_t)a.pages % 16 == 0 && (a.q_dtype != ECHOKV_F32 || L->head_size < 256);
+  return mfma ? ek::launch_prefix(a, s) : ek::launch_prefix_any(a, s);
 }
 
 }  // namespace
@@ -736,9 +753,9 @@ int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* b
     a.p_s0 = p_s0;
     a.p_s1 = p_s1;
     a.lse = lse;
-    return launched(ek::launch_prefix_any(a, (hipStream_t)stream));
+    return launched(run_prefix(L, a, (hipStream_t)stream));
   }
-  if (ek::launch_prefix_any(a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
+  if (run_prefix(L, a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
   const ek::JoinArgs j{a.acc, a.ml, ranges, nullptr, nullptr, nullptr, 0, ek::Splits{}, nullptr, 0, L->block_size,
                        q_rows, n, num_q_heads, L->head_size, part, p_s0, p_s1, ECHOKV_F32, lse};
   return launched(ek::launch_join(j, (hipStream_t)stream));
@@ -776,7 +793,7 @@ int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int
                                  num_seqs, blocks, prefix_len, softmax_scale, ranges, rows);
   a.lens = seq_lens;
   a.suffix = suffix;
-  if (ek::launch_prefix_any(a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
+  if (run_prefix(L, a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
   float* acc = rows + ranges * num_seqs * num_q_heads * (L->head_size + 2);
   float* ml = acc + num_splits * num_seqs * num_q_heads * L->head_size;
   ek::JoinArgs j{a.acc, a.ml, ranges, nullptr, nullptr, suffix, num_splits, ek::Splits{}, seq_lens, (int)prefix_len,

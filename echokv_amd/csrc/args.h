@@ -409,7 +409,12 @@ struct PrefixArgs {
   // written for the kernels that follow.
   const int64_t* lens;
   int64_t* suffix;
+  // The 16-bit kernel's: log2 of block size and K group, and page = umulhi(chunk id, kc_mul)
+  // (0: one chunk a page).
+  int bs_shift, kg_shift;
+  uint32_t kc_mul;
 };
+constexpr int kPrefixRows = 128;  // query rows of a workgroup: 32 for each of the 16-bit kernel's four waves
 
 // The ranges of the prefix and, in decode, the splits of the suffixes, added and normalized.
 struct JoinArgs {
@@ -485,6 +490,7 @@ hipError_t launch_prefill_flash(const FlashArgs& a, hipStream_t s);
 bool prompt_mfma(const PromptArgs& a);  // whether the 16-bit kernel takes the call
 hipError_t launch_prompt(const PromptArgs& a, hipStream_t s);
 hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s);
+hipError_t launch_prefix(const PrefixArgs& a, hipStream_t s);
 hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s);
 hipError_t launch_join(const JoinArgs& a, hipStream_t s);
 

@@ -140,8 +140,6 @@ def check_decode(c, q, got, lens, scale, rows=None):
         k, v = c.tokens(i, n)
         j = i if rows is None else rows[i]
         r = Rows(q[j : j + 1], k, v, [n], scale)
-        # The decode kernels' own error is within 2e-3 of their budget; weights and values here
-        # as in BOUND.
         check(got[j : j + 1], r, **BOUND)
 
 
@@ -174,7 +172,11 @@ def test_decode_batches(device, seqs, prefix):
     torch.cuda.synchronize()
     assert got.dtype == torch.float32
     check_decode(c, q, got, c.lens, c.d ** -0.5)
-    assert float((got - plain).abs().max()) <= 4e-3  # both within 2e-3
+    # Plain decode is within 2e-3 of the exact result, this one within its bound: they differ by
+    # both at most. (2e-3 does not hold here: values reach 40, where float16's half step is 2^-7.)
+    for i, n in enumerate(c.lens):
+        r = Rows(q[i : i + 1], *c.tokens(i, n), [n], c.d ** -0.5)
+        assert ((got[i : i + 1] - plain[i : i + 1]).abs().double() <= r.bound(F32, **BOUND) + 2e-3).all()
 
 
 def test_decode_rows_of_other_sequences_stay(device):
