@@ -663,9 +663,9 @@ bool prefix_mfma(const echokv_layout* L) {
 // Ranges of a shared prefix: enough workgroups for the chip (two for each of its 256
 // CUs) with at least 128 keys each.
 int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
-  const int64_t gqa = hq / L->num_kv_heads, rows = prefix_mfma(L) ? ek::kPrefixRows : 64;
-  const int64_t wgs = (n * gqa + rows - 1) / rows * L->num_kv_heads;
-  int64_t r = (512 + wgs - 1) / wgs;
+  const int64_t n_rows = n * (hq / L->num_kv_heads), rows = prefix_mfma(L) ? ek::prefix_rows(L->head_size, ECHOKV_F16, n_rows) : 64;
+  const int64_t wgs = (n_rows + rows - 1) / rows * L->num_kv_heads;
+  int64_t r = ((rows == 256 ? 256 : 512) + wgs - 1) / wgs;
   const int64_t most = len / 128;
   r = r < most ? r : most;
   return (int)(r < 1 ? 1 : r < 64 ? r : 64);

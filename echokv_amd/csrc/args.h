@@ -414,7 +414,11 @@ struct PrefixArgs {
   int bs_shift, kg_shift;
   uint32_t kc_mul;
 };
-constexpr int kPrefixRows = 128;  // query rows of a workgroup: 32 for each of the 16-bit kernel's four waves
+// Query rows of a workgroup of the 16-bit kernel: 32 per wave, four waves or (16-bit queries up to
+// head size 128, more than 128 rows) eight.
+inline int prefix_rows(int head_size, int q_dtype, int64_t rows) {
+  return head_size <= 128 && q_dtype != ECHOKV_F32 && rows > 128 ? 256 : 128;
+}
 
 // The ranges of the prefix and, in decode, the splits of the suffixes, added and normalized.
 struct JoinArgs {

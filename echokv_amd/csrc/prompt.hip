@@ -25,9 +25,8 @@ constexpr float kInf = __builtin_inff();
 
 template <int D>
 struct Ring {
-  static constexpr int SIDE = kKeys * D * 2;  // bytes of a step's keys, then its values
-  static constexpr int STEP = 2 * SIDE;
-    static constexpr int NDMA = STEP / 1024 / kWaves;
+  static constexpr int SIDE = kKeys * D * 2;  // bytes of a step's keys (its values take as many)
+  static constexpr int NDMA = SIDE / 1024 / kWaves;
 };
 
 }  // namespace
@@ -37,7 +36,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
   using R = Ring<D>;
   constexpr int NS = D / 16, NDB = D / 32, NDMA = R::NDMA;
   constexpr uint32_t kTop = BF ? 0x7f80u : 0x7c00u;  // infinity's bits
-  constexpr float kShift = BF ? 0.f : 6.f;  // float16 weights are 2^6 times the softmax's
   extern __shared__ __attribute__((aligned(1024))) uint8_t ring[];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -57,190 +55,140 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
   const int first_pos = t0 + 32 * wave / a.gqa;                              // the wave's first row's
   const int last_pos = t0 + min(32 * wave + 31, n_rows - 1) / a.gqa;  // and last row's position
 
-  // This lane's share of a step's loads: byte offsets from the step's first key row. The
-  // permutation of LDS slots is made on the memory side, since LDS fills in lane order.
-  const uint32_t k_row = (uint32_t)a.k_s0 * 2, v_row = (uint32_t)a.v_s0 * 2;
+  // LDS: the keys of two steps, then the values of two. This lane's share of a step's loads: byte
+  // offsets from the step's first row. The permutation of LDS slots is made on the memory side,
+  // since LDS fills in lane order.
   const uint8_t* kbase = (const uint8_t*)a.k + 2 * (row0 * a.k_s0 + (long)h * a.k_s1);
   const uint8_t* vbase = (const uint8_t*)a.v + 2 * (row0 * a.v_s0 + (long)h * a.v_s1);
   const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
-  auto issue = [&](int step) {
-    const int kb = step * kKeys;
-    const uint8_t* kg = uniform_ptr(kbase + (long)kb * a.k_s0 * 2);
-    const uint8_t* vg = uniform_ptr(vbase + (long)kb * a.v_s0 * 2);
-    const uint32_t to = ring0 + (uint32_t)((step % kSlots) * R::STEP + 1024 * NDMA * wave);
-    const int last = kv_end - 1 - kb;
+  auto issue = [&](int step, bool val) {
+    const int kb = step * kKeys, last = kv_end - 1 - kb;
+    const uint32_t stride = (uint32_t)(val ? a.v_s0 : a.k_s0) * 2;
+    const uint8_t* from = uniform_ptr((val ? vbase : kbase) + (long)kb * stride);
+    const uint32_t to = ring0 + (uint32_t)(((val ? kSlots : 0) + step % kSlots) * R::SIDE + 1024 * NDMA * wave);
 #pragma unroll
     for (int i = 0; i < NDMA; ++i) {
-      const int p = 1024 * (NDMA * wave + i);
-      const bool val = p >= R::SIDE;  // wave-uniform
-      const int q = (p & (R::SIDE - 1)) + 16 * lane;
+      const int q = 1024 * (NDMA * wave + i) + 16 * lane;
       const int key = q / (2 * D), slot = q % (2 * D) / 16;
-      const int row = min(key, last);
-      const uint32_t off = (uint32_t)row * (val ? v_row : k_row) + 16 * (slot ^ (val ? v_swz<D>(key) : k_swz<D>(key)));
-      dma16(val ? vg : kg, off, to + 1024 * i);
+      const uint32_t off = (uint32_t)min(key, last) * stride + 16 * (slot ^ (val ? v_swz<D>(key) : k_swz<D>(key)));
+      dma16(from, off, to + 1024 * i);
     }
   };
-#pragma unroll
-  for (int i = 0; i < kSlots - 1; ++i)
-    if (i < n_steps) issue(i);
+  issue(0, false);
+  issue(0, true);
+  if (n_steps > 1) issue(1, false);
 
-  // Query fragments (B operand): row r, channels 16 s + 8 hh .. + 8. Scores are scaled inside
-  // the exponent and their maximum is taken before, which needs the scale positive: a negative
-  // one flips the query's sign, a zero one becomes 2^-100.
-  constexpr float kTiny = 7.8886090522101181e-31f;
-  const float scale = fabsf(a.scale_log2) < kTiny ? kTiny : fabsf(a.scale_log2);  // NaN stays
-  h8_t q[NS];
+  // Query fragments (B operand): row r, channels 16 s + 8 hh .. + 8.
+  Rows<D, BF, 2, 1, false> w;
+  w.set_scale(a.scale_log2);
   {
     const uint16_t* src = (const uint16_t*)a.q + (row0 + pos) * a.q_s0 + (long)qh * a.q_s1 + 8 * hh;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) q[s] = *(const h8_t*)(src + 16 * s);
+    for (int s = 0; s < NS; ++s) w.q[s] = *(const h8_t*)(src + 16 * s);
     if (a.scale_log2 < 0.f) {
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        u4_t w = __builtin_bit_cast(u4_t, q[s]);
-        w ^= 0x80008000u;
-        q[s] = __builtin_bit_cast(h8_t, w);
-      }
+      for (int s = 0; s < NS; ++s)
+        w.q[s] = __builtin_bit_cast(h8_t, __builtin_bit_cast(u4_t, w.q[s]) ^ 0x80008000u);
     }
   }
 
-  f16v_t acc[NDB];
-  float m_run, lsum;
-  auto clear = [&]() {
-#pragma unroll
-    for (int db = 0; db < NDB; ++db) acc[db] = f16v_t{};
-    m_run = -kInf;
-    lsum = 0.f;
-  };
-  // Scores of the step at key kb0 to rounded weights (p[ks]: 16 keys), online. `edge`: some row
-  // does not see the whole step.
-  auto softmax = [&](f16v_t* s, int kb0, bool edge, u4_t* p) {
-    if (edge) {
-      const int left = pos - kb0 - 4 * hh;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) > left ? -kInf : s[kb][i];
-    }
-    float mx = -kInf;
+  // Scores of keys behind the row's position: -inf. `edge`: some row does not see the whole step.
+  auto mask = [&](int kb0, f16v_t* s) {
+    int left = pos - kb0 - 4 * hh;
+    asm volatile("" : "+v"(left));  // keeps the compares in this branch
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    const float mt = halves_max(mx) * scale;
-    // The running maximum moves only when a row's passes it by more than 2^8: weights stay
-    // below 2^8 meanwhile.
-    if (__builtin_amdgcn_ballot_w64(mt > m_run + 8.f)) {
-      const float m_new = fmaxf(m_run, mt);
-      const float alpha = m_new == -kInf ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-      lsum *= alpha;
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
-      m_run = m_new;
-    }
-    const float ms = m_run == -kInf ? 0.f : m_run - kShift;
-    float sum[2] = {0.f, 0.f};
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], scale, -ms));
-        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], scale, -ms));
-        sum[0] += x;
-        sum[1] += y;
-        p[2 * kb + (i >> 3)][(i & 7) >> 1] = pack2<BF>(x, y);
-      }
-    lsum += sum[0] + sum[1];
+      for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) > left ? -kInf : s[kb][i];
   };
+  auto edge_of = [&](int step) { return (step + 1) * kKeys > first_pos + 1; };
 
-  uint32_t k_lane[NS], v_lane[NDB];
-#pragma unroll
-  for (int c = 0; c < NS; ++c) k_lane[c] = k_at<D>(c, j, hh);
-#pragma unroll
-  for (int db = 0; db < NDB; ++db) v_lane[db] = v_at<D>(db, lane);
-  clear();
+  w.clear();
+  const uint32_t k_lane = ring0 + k_at<D>(0, j, hh), v_lane = ring0 + kSlots * R::SIDE + v_at<D>(0, lane);
+  const int my_steps = active ? last_pos / kKeys + 1 : 0;  // steps that some row of the wave sees
   bool odd = false;  // a step with an edge holds an infinite value or NaN
-  for (int step = 0; step < n_steps; ++step) {
-    // This wave's share of the step has landed, with the barrier every wave's; its loads were made a
-    // step ago, and the next step's go to the slot that every wave has left.
+  // This wave's loads have landed, with the barrier every wave's: the keys of `step` + 1 and the
+  // values of `step`. They were made a step ago; the next ones go to the slots that every wave has
+  // left.
+  auto advance = [&](int step) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (step + kSlots - 1 < n_steps) issue(step + kSlots - 1);
-    const int kb0 = step * kKeys;
-    if (!active || odd || kb0 > last_pos) continue;
-    const uint32_t kt = ring0 + (uint32_t)((step % kSlots) * R::STEP);
-
-    // Fragments two contraction steps at a time, the next ones requested before the products of
-    // the current (scheduling fences keep that order, and their registers).
-    f16v_t s[2] = {f16v_t{}, f16v_t{}};
-    {
-      h8_t f[2][4];
-      auto load = [&](int g, h8_t* x) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = k_read<D>(k_lane[2 * g + (i >> 1)] + kt, i & 1);
-      };
-      load(0, f[0]);
-#pragma unroll
-      for (int g = 0; g < NS / 2; ++g) {
-        if (g + 1 < NS / 2) load(g + 1, f[(g + 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[i & 1] = mma<BF>(f[g & 1][i], q[2 * g + (i >> 1)], s[i & 1]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    const bool edge = kb0 + kKeys > first_pos + 1;
-    if (edge) {
-      typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
-      us2_t m = {0, 0};
+    if (step + 2 < n_steps) issue(step + 2, false);
+    if (step + 1 < n_steps) issue(step + 1, true);
+  };
+  auto vslot = [&](int step) { return (uint32_t)(step % kSlots * R::SIDE); };
+  auto look = [&](int step) {
+    if (!edge_of(step)) return;
+    typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
+    us2_t m = {0, 0};
+    const uint32_t vt = ring0 + kSlots * R::SIDE + vslot(step) + 16 * lane;
 #pragma unroll 4
-      for (int i = 0; i < R::SIDE / 1024; ++i) {
-        const u4_t w = *(const lds_t<u4_t>*)(kt + R::SIDE + 1024 * i + 16 * lane);
+    for (int i = 0; i < R::SIDE / 1024; ++i) {
+      const u4_t x = *(const lds_t<u4_t>*)(vt + 1024 * i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2_t, w[e] & 0x7fff7fffu));
-      }
-      odd = __builtin_amdgcn_ballot_w64(m[0] >= kTop || m[1] >= kTop);
+      for (int e = 0; e < 4; ++e) m = __builtin_elementwise_max(m, __builtin_bit_cast(us2_t, x[e] & 0x7fff7fffu));
     }
+    odd = odd || __builtin_amdgcn_ballot_w64(m[0] >= kTop || m[1] >= kTop);
+  };
+  f16v_t s0[2], s1[2];
+  float mt = -kInf;
+  // A step's weights and values beside the next step's scores (tiles.h).
+  auto body = [&](int step, f16v_t* cur, f16v_t* nxt) {
+    advance(step);
+    look(step);
+    w.rescale(mt);
     u4_t p[4];
-    softmax(s, kb0, edge, p);
-    {
-      constexpr int NG = NDB < 4 ? NDB : 4, NP = NDB / NG;  // channel blocks of a group, groups of 16 keys
-      h8_t f[2][NG];
-      auto load = [&](int g, h8_t* x) {
-#pragma unroll
-        for (int i = 0; i < NG; ++i) x[i] = v_read<D>(v_lane[g % NP * NG + i] + kt + R::SIDE, g / NP);
-      };
-      load(0, f[0]);
-#pragma unroll
-      for (int g = 0; g < 4 * NP; ++g) {
-        if (g + 1 < 4 * NP) load(g + 1, f[(g + 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          const int db = g % NP * NG + i;
-          acc[db] = mma<BF>(f[g & 1][i], __builtin_bit_cast(h8_t, p[g / NP]), acc[db]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    w.template weights<true, R::SIDE>(cur, p, k_lane + (uint32_t)((step + 1) % kSlots * R::SIDE), nxt);
+    mt = w.template values<true>(p, v_lane + vslot(step), nxt);
+    if (edge_of(step + 1)) {
+      mask((step + 1) * kKeys, nxt);
+      mt = w.top(nxt);
     }
+  };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int step = 0;
+  if (my_steps > 0) {
+    w.template scores<R::SIDE>(k_lane, s0);
+    if (edge_of(0)) mask(0, s0);
+    mt = w.top(s0);
+    for (; step + 2 < my_steps; step += 2) {
+      body(step, s0, s1);
+      body(step + 1, s1, s0);
+    }
+    if (step + 1 < my_steps) {
+      body(step++, s0, s1);
+      s0[0] = s1[0];
+      s0[1] = s1[1];
+    }
+    advance(step);
+    look(step);
+    w.rescale(mt);
+    u4_t p[4];
+    w.template weights<false, R::SIDE>(s0, p, 0, s0);
+    w.template values<false>(p, v_lane + vslot(step), s0);
+    ++step;
   }
+  for (; step < n_steps; ++step) advance(step);  // steps of the workgroup's later rows
 
   // Rare: the wave's rows once more, from memory. The products leave infinite values and NaN out;
   // which of them a row sees is a product of its own, of 0 / 1 weights with 1 for +inf, 2^7 for
   // -inf and 2^14 for NaN (at most 64 of each a step: the sum tells them apart).
   if (odd) {
-    clear();
+    w.clear();
 #pragma unroll 1
     for (int kb0 = 0; kb0 <= last_pos; kb0 += kKeys) {
-      f16v_t s[2] = {f16v_t{}, f16v_t{}};
+      f16v_t x2[2] = {f16v_t{}, f16v_t{}};
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         const uint8_t* row = kbase + 2 * (long)min(kb0 + 32 * kb + j, kv_end - 1) * a.k_s0 + 16 * hh;
 #pragma unroll
-        for (int c = 0; c < NS; ++c) s[kb] = mma<BF>(*(const h8_t*)(row + 32 * c), q[c], s[kb]);
+        for (int c = 0; c < NS; ++c) x2[kb] = mma<BF>(*(const h8_t*)(row + 32 * c), w.q[c], x2[kb]);
       }
+      mask(kb0, x2);
+      w.rescale(w.top(x2));
       u4_t p[4];
-      softmax(s, kb0, true, p);
+      w.template weights<false, R::SIDE>(x2, p, 0, x2);
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks) {
         uint32_t seen[4];
@@ -253,7 +201,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
         }
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
-          u4_t w, kinds;
+          u4_t val, kinds;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t x[2], k[2];
@@ -265,10 +213,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
               k[u] = bad ? k[u] : 0;
               x[u] = bad ? 0 : x[u];
             }
-            w[e] = x[0] | x[1] << 16;
+            val[e] = x[0] | x[1] << 16;
             kinds[e] = k[0] | k[1] << 16;
           }
-          acc[db] = mma<BF>(__builtin_bit_cast(h8_t, w), __builtin_bit_cast(h8_t, p[ks]), acc[db]);
+          w.acc[db] = mma<BF>(__builtin_bit_cast(h8_t, val), __builtin_bit_cast(h8_t, p[ks]), w.acc[db]);
           f16v_t found = f16v_t{};
           found = mma<BF>(__builtin_bit_cast(h8_t, kinds), __builtin_bit_cast(h8_t, u4_t{seen[0], seen[1], seen[2], seen[3]}),
                           found);
@@ -277,7 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
             const int n = (int)found[i];
             float x = n & 127 ? kInf : 0.f;
             x = n >> 7 & 127 ? (n & 127 ? __builtin_nanf("") : -kInf) : x;
-            acc[db][i] += n >> 14 ? __builtin_nanf("") : x;
+            w.acc[db][i] += n >> 14 ? __builtin_nanf("") : x;
           }
           __builtin_amdgcn_sched_barrier(0);
         }
@@ -285,10 +233,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
     }
   }
 
-  const float l = halves_sum(lsum);
+  const float l = halves_sum(w.l);
   if (!live) return;
   const long row = row0 + pos, lr = row * a.hq + qh;
-  float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -kInf : m_run - kShift + __log2f(l), wp = 0.f;
+  float inv = l == 0.f ? 0.f : 1.f / l, lse = l == 0.f ? -kInf : w.m - w.kShift + __log2f(l), wp = 0.f;
   if (a.part) {
     const float pl = a.part_lse[lr], mx = fmaxf(pl, lse);
     if (mx != -kInf) {
@@ -300,7 +248,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
   }
   if (a.lse && hh == 0) a.lse[lr] = lse;
 #pragma unroll
-  for (int db = 0; db < NDB; ++db) acc[db] *= inv;
+  for (int db = 0; db < NDB; ++db) w.acc[db] *= inv;
   if (wp != 0.f) {
     const float* src = a.part + row * a.p_s0 + (long)qh * a.p_s1 + 4 * hh;
 #pragma unroll
@@ -309,7 +257,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
       for (int g = 0; g < 4; ++g) {
         const f4_t x = *(const f4_any_t*)(src + 32 * db + 8 * g);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[db][4 * g + e] = __builtin_fmaf(wp, x[e], acc[db][4 * g + e]);
+        for (int e = 0; e < 4; ++e) w.acc[db][4 * g + e] = __builtin_fmaf(wp, x[e], w.acc[db][4 * g + e]);
       }
   }
   const long ob = row * a.o_s0 + (long)qh * a.o_s1;
@@ -319,11 +267,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void prompt_kernel(P
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g)
-        *(f4_any_t*)(dst + 32 * db + 8 * g) = f4_t{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+        *(f4_any_t*)(dst + 32 * db + 8 * g) = f4_t{w.acc[db][4 * g], w.acc[db][4 * g + 1], w.acc[db][4 * g + 2], w.acc[db][4 * g + 3]};
   } else if (a.out_dtype == ECHOKV_BF16) {
-    store16<NDB, true>((uint8_t*)a.out + 2 * ob, acc, hh);
+    store16<NDB, true>((uint8_t*)a.out + 2 * ob, w.acc, hh);
   } else {
-    store16<NDB, false>((uint8_t*)a.out + 2 * ob, acc, hh);
+    store16<NDB, false>((uint8_t*)a.out + 2 * ob, w.acc, hh);
   }
 }
 
@@ -340,7 +288,7 @@ bool prompt_mfma(const PromptArgs& a) {
 template <int D, bool BF>
 static hipError_t launch_t(const PromptArgs& a, hipStream_t s) {
   using R = Ring<D>;
-  constexpr int lds = kSlots * R::STEP;
+  constexpr int lds = 2 * kSlots * R::SIDE;
   static std::atomic<uint64_t> attr_done{0};
   const hipError_t e = ensure_lds_limit((const void*)prompt_kernel<D, BF>, lds, &attr_done);
   if (e != hipSuccess) return e;

@@ -28,20 +28,24 @@ struct Raw {
 
 }  // namespace
 
-template <int D, bool QLO>
-__global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2) void prefix_kernel(PrefixArgs a) {
+template <int D, bool QLO, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) void prefix_kernel(PrefixArgs a) {
+  static_assert(WAVES == 4 || WAVES == 8, "a thread takes its items' K and V, or one of them");
+  constexpr bool BOTH = WAVES == 4;
+  constexpr int BUFS = BOTH ? 1 : 2;        // steps in LDS
+  constexpr int ROWS = 32 * WAVES;
   constexpr int KEYS = 8192 / D;            // keys per step: 256 items
   constexpr int NKB = KEYS >= 64 ? 2 : 1;   // 32-key blocks per softmax update
   constexpr int NS = D / 16, NDB = D / 32, OCTS = D / 8;
   constexpr int SIDE = KEYS * D * 2;        // bytes of K hi, then K lo, then V
   constexpr float kShift = 6.f;             // weights are 2^6 times the softmax's: small ones keep their bits
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[3 * SIDE];
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const Lay& L = a.L;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int tid = threadIdx.x, j = lane & 31, hh = lane >> 5;
   if (a.suffix)
-    for (int t = (int)blockIdx.x * 256 + tid; t < a.n; t += (int)gridDim.x * 256) {
+    for (int t = (int)blockIdx.x * 64 * WAVES + tid; t < a.n; t += (int)gridDim.x * 64 * WAVES) {
       const long x = a.lens[t] - a.len;
       a.suffix[t] = x > 0 ? x : 0;
     }
@@ -53,7 +57,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
   const int n_steps = k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
 
   // ---- this thread's item of a step, and its chain of loads ----------------
-  const int oct = tid % OCTS, quad = tid / OCTS;
+  const int oct = tid % OCTS, quad = tid % 256 / OCTS;
+  const bool keys = BOTH || wave < 4, values = BOTH || wave >= 4;  // wave-uniform: what of the item this thread takes
   const int ch = 8 * oct;
   const int G = D / L.VG, vg = ch / L.VG;
   // Nothing loaded is looked at before the step that needs it, and no load sits in a
@@ -95,23 +100,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
     // A quad that cannot be read takes its page's first bytes instead (dequantized to zero).
     const uint8_t* kp = ok ? a.pages + cb + (long)(off & ((1 << tpc_shift) - 1)) * rowb + ((h * D + ch) * bits / 8 & ~7) : pg;
     const int step_b = ok ? rowb : 0;
+    if (keys) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w.k[i] = *(const uint2*)(kp + i * step_b);
-      w.v[i] = *(const uint2*)(kp + i * step_b + step_b / 2);
+      for (int i = 0; i < 4; ++i) w.k[i] = *(const uint2*)(kp + i * step_b);
+      const int se = ((off >> a.kg_shift) * L.H + h) * D + ch;
+      w.ks = *(const uint4*)(pg + L.o_ks + 2 * se);
+      w.km = *(const uint4*)(pg + L.o_km + 2 * se);
     }
-    const int se = ((off >> a.kg_shift) * L.H + h) * D + ch;
-    w.ks = *(const uint4*)(pg + L.o_ks + 2 * se);
-    w.km = *(const uint4*)(pg + L.o_km + 2 * se);
-    const int ve = (off * L.H + h) * G + vg;
+    if (values) {
+      const int ve = (off * L.H + h) * G + vg;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w.vs[i] = *(const uint16_t*)(pg + L.o_vs + 2 * (ve + i * L.H * G));
-      w.vm[i] = *(const uint16_t*)(pg + L.o_vm + 2 * (ve + i * L.H * G));
+      for (int i = 0; i < 4; ++i) {
+        (BOTH ? w.v : w.k)[i] = *(const uint2*)(kp + i * step_b + step_b / 2);
+        w.vs[i] = *(const uint16_t*)(pg + L.o_vs + 2 * (ve + i * L.H * G));
+        w.vm[i] = *(const uint16_t*)(pg + L.o_vm + 2 * (ve + i * L.H * G));
+      }
     }
   };
   // The item dequantized into LDS (keys past the range and blocks that cannot be read: zeros).
   auto store_item = [&](int step, const Head& x, const Raw& w) {
+    uint8_t* const buf = lds + (BOTH ? 0 : (step & 1) * 3 * SIDE);
     const int kp = item_key(step), off = item_off(step), bits = tier_of(x.h.x & 0xffu);
     const int key0 = 4 * quad;
     auto put_k = [&](int i, const float* x8) {
@@ -123,32 +131,41 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
         lo[e] = pack2<false>(x8[2 * e] - (float)p[0], x8[2 * e + 1] - (float)p[1]);
       }
       const int at = (key0 + i) * (2 * D) + 16 * (oct ^ k_swz<D>(key0 + i));
-      *(u4_t*)(lds + at) = hi;
-      *(u4_t*)(lds + SIDE + at) = lo;
+      *(u4_t*)(buf + at) = hi;
+      *(u4_t*)(buf + SIDE + at) = lo;
     };
     auto put_v = [&](int i, const u4_t x) {
-      *(u4_t*)(lds + 2 * SIDE + (key0 + i) * (2 * D) + 16 * (oct ^ v_swz<D>(key0 + i))) = x;
+      *(u4_t*)(buf + 2 * SIDE + (key0 + i) * (2 * D) + 16 * (oct ^ v_swz<D>(key0 + i))) = x;
     };
     const int sh = 8 * (((h * D + ch) * bits / 8) & 7);
     auto rows = [&](auto width) {
       constexpr int B = decltype(width)::value;
       const uint32_t sw[4] = {w.ks.x, w.ks.y, w.ks.z, w.ks.w}, mw[4] = {w.km.x, w.km.y, w.km.z, w.km.w};
+      if (keys) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        h2_t c[4];
-        code_pairs<B>(w.k[i], sh, c);
-        float x8[8];
+        for (int i = 0; i < 4; ++i) {
+          h2_t c[4];
+          code_pairs<B>(w.k[i], sh, c);
+          float x8[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          x8[e] = __builtin_fmaf((float)c[e >> 1][e & 1], (float)u2h(sw[e >> 1])[e & 1], (float)u2h(mw[e >> 1])[e & 1]);
-        put_k(i, x8);
-        code_pairs<B>(w.v[i], sh, c);
-        const h2_t vs = u2h(w.vs[i] * 0x10001u), vm = u2h(w.vm[i] * 0x10001u);
-        u4_t v;
+          for (int e = 0; e < 8; ++e)
+            x8[e] = __builtin_fmaf((float)c[e >> 1][e & 1], (float)u2h(sw[e >> 1])[e & 1], (float)u2h(mw[e >> 1])[e & 1]);
+          put_k(i, x8);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (values) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[e], vs, vm));
-        put_v(i, v);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < 4; ++i) {
+          h2_t c[4];
+          code_pairs<B>((BOTH ? w.v : w.k)[i], sh, c);
+          const h2_t vs = u2h(w.vs[i] * 0x10001u), vm = u2h(w.vm[i] * 0x10001u);
+          u4_t v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[e], vs, vm));
+          put_v(i, v);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     };
     if (bits == 4) rows(std::integral_constant<int, 4>{});
@@ -159,11 +176,11 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
       const float z8[8] = {};
 #pragma unroll 1
       for (int i = n_live > 0 ? n_live : 0; i < 4; ++i) {
-        put_k(i, z8);
-        put_v(i, u4_t{});
+        if (keys) put_k(i, z8);
+        if (values) put_v(i, u4_t{});
       }
     }
-    if (w.ok && (unsigned)x.rs < (unsigned)a.res.rows && w.rg == off >> a.kg_shift) {  // rare: an open K group
+    if (keys && w.ok && (unsigned)x.rs < (unsigned)a.res.rows && w.rg == off >> a.kg_shift) {  // rare: an open K group
 #pragma unroll 1
       for (int i = 0; i < 4 && kp + i < k_end; ++i) {
         float x8[8];
@@ -191,12 +208,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
     bool live;
   };
   auto row_of = [&](int jj) {
-    const int r = tile * kPrefixRows + 32 * wave + jj;
+    const int r = tile * ROWS + 32 * wave + jj;
     const bool live = r < n_rows;
     const int t = live ? (int)((unsigned)r / (unsigned)a.gqa) : 0;
     return Row{t, h * a.gqa + (live ? r - t * a.gqa : 0), a.q_rows ? a.q_rows[t] : t, live};
   };
-  const bool active = tile * kPrefixRows + 32 * wave < n_rows;
+  const bool active = tile * ROWS + 32 * wave < n_rows;
   // As in prompt.hip: the scale positive.
   constexpr float kTiny = 7.8886090522101181e-31f;
   const float scale = fabsf(a.scale_log2) < kTiny ? kTiny : fabsf(a.scale_log2);
@@ -239,17 +256,33 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
   // fragment's address is the first one's with the slot's bits flipped.
   const uint32_t k_lane = lds0 + k_at<D>(0, j, hh), v_lane = lds0 + 2 * SIDE + v_at<D>(0, lane);
 
-  for (int step = 0; step < n_steps; ++step) {
-    __syncthreads();  // every wave is done with the step before
+  // An item into LDS, then the words of the next one requested.
+  auto put_step = [&](int step) {
     store_item(step, head, raw);
-    __syncthreads();
     if (step + 1 < n_steps) {
       head = head1;
       load_raw(step + 1, head, raw);
       head1 = load_head(blk2);
       blk2 = load_blk(step + 3);
     }
+  };
+  if (!BOTH && n_steps > 0) put_step(0);
+  for (int step = 0; step < n_steps; ++step) {
+    __syncthreads();  // every wave is done with the step before (eight waves: and this one is there)
+    if constexpr (BOTH) {
+      store_item(step, head, raw);
+      __syncthreads();
+      if (step + 1 < n_steps) {
+        head = head1;
+        load_raw(step + 1, head, raw);
+        head1 = load_head(blk2);
+        blk2 = load_blk(step + 3);
+      }
+    } else if (step + 1 < n_steps) {
+      put_step(step + 1);
+    }
     if (!active) continue;
+    const uint32_t buf = BOTH ? 0u : (uint32_t)((step & 1) * 3 * SIDE);
 #pragma unroll 1
     for (int sb = 0; sb < KEYS; sb += 32 * NKB) {
       const int left = k_end - (k_begin + step * KEYS + sb);  // keys of this block that there are
@@ -262,7 +295,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
         auto load = [&](int u, h8_t* x) {  // channels 16 (u / 2) .. + 16 of K hi or lo
 #pragma unroll
           for (int kb = 0; kb < NKB; ++kb)
-            x[kb] = k_read<D>((k_lane ^ 32 * (u >> 1)) + (u & 1) * SIDE + sb * 2 * D, kb);
+            x[kb] = k_read<D>((k_lane ^ 32 * (u >> 1)) + (u & 1) * SIDE + buf + sb * 2 * D, kb);
         };
         load(0, f[0]);
 #pragma unroll
@@ -321,7 +354,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
         h8_t f[2][NG];
         auto load = [&](int g, h8_t* x) {
 #pragma unroll
-          for (int i = 0; i < NG; ++i) x[i] = v_read<D>((v_lane ^ 64 * (g % NP * NG + i)) + sb * 2 * D, g / NP);
+          for (int i = 0; i < NG; ++i) x[i] = v_read<D>((v_lane ^ 64 * (g % NP * NG + i)) + buf + sb * 2 * D, g / NP);
         };
         load(0, f[0]);
 #pragma unroll
@@ -361,16 +394,26 @@ __global__ __launch_bounds__(64 * kWaves, D == 256 || (QLO && D == 128) ? 1 : 2)
   }
 }
 
+template <int D, bool QLO, int WAVES>
+static hipError_t launch_t(const PrefixArgs& a, hipStream_t s) {
+  constexpr int lds = (WAVES == 8 ? 2 : 1) * 3 * 8192 * 2;
+  static std::atomic<uint64_t> attr_done{0};
+  const hipError_t e = ensure_lds_limit((const void*)prefix_kernel<D, QLO, WAVES>, lds, &attr_done);
+  if (e != hipSuccess) return e;
+  constexpr int rows = 32 * WAVES;
+  const dim3 grid((unsigned)((a.n * a.gqa + rows - 1) / rows * a.L.H), (unsigned)a.ranges);
+  hipLaunchKernelGGL((prefix_kernel<D, QLO, WAVES>), grid, dim3(64 * WAVES), lds, s, a);
+  return hipGetLastError();
+}
+
 template <int D>
 static hipError_t launch_d(const PrefixArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((a.n * a.gqa + kPrefixRows - 1) / kPrefixRows * a.L.H), (unsigned)a.ranges);
   if (a.q_dtype == ECHOKV_F32) {
     if constexpr (D == 256) return hipErrorInvalidValue;  // its registers do not fit: attend_any.hip
-    else hipLaunchKernelGGL((prefix_kernel<D, true>), grid, dim3(64 * kWaves), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((prefix_kernel<D, false>), grid, dim3(64 * kWaves), 0, s, a);
+    else return launch_t<D, true, 4>(a, s);
   }
-  return hipGetLastError();
+  if constexpr (D == 256) return launch_t<D, false, 4>(a, s);
+  else return prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa) == 256 ? launch_t<D, false, 8>(a, s) : launch_t<D, false, 4>(a, s);
 }
 
 hipError_t launch_prefix(const PrefixArgs& a, hipStream_t s) {

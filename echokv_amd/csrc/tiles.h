@@ -105,6 +105,156 @@ __device__ __forceinline__ h8_t v_read(uint32_t at, int ks) {
   return __builtin_bit_cast(h8_t, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// One wave's 32 rows over steps of 32 NKB keys. The loop is skewed by a step so that matrix and
+// vector instructions run side by side in one wave (apart, a wave's products wait for its
+// exponentials and back, and two waves a SIMD did not fill the gaps): the exponentials of step i
+// go between the score products of step i + 1, whose maxima go between the value products of
+// step i. Scheduling fences hold that order.
+//
+// PARTS: keys as one matrix or as hi + lo, `side` bytes apart. QLO: the queries as hi + lo too.
+template <int D, bool BF, int NKB, int PARTS, bool QLO>
+struct Rows {
+  static constexpr int NS = D / 16, NDB = D / 32;
+  static constexpr int NP = 8 * NKB;  // pairs of scores a lane
+  static constexpr float kShift = BF ? 0.f : 6.f;  // float16 weights are 2^6 times the softmax's: small ones keep their bits
+  static constexpr float kInf = __builtin_inff();
+  h8_t q[NS], ql[QLO ? NS : 1];
+  f16v_t acc[NDB];
+  float m, l;      // running maximum (log2 units), this lane's share of the sum
+  float scale;     // softmax scale in log2 units, positive
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int db = 0; db < NDB; ++db) acc[db] = f16v_t{};
+    m = -kInf;
+    l = 0.f;
+  }
+  // Scores are scaled inside the exponent and their maximum is taken before, which needs the scale
+  // positive: a negative one flips the query's sign (the caller's), a zero one becomes 2^-100.
+  __device__ __forceinline__ void set_scale(float s) {
+    constexpr float kTiny = 7.8886090522101181e-31f;
+    scale = fabsf(s) < kTiny ? kTiny : fabsf(s);  // NaN stays
+  }
+
+  // Fragments are requested AHEAD products before theirs, into a ring.
+  static constexpr int UNITS = NS * PARTS * NKB, RING = 4, AHEAD = RING - 1;
+  template <int SIDE>
+  __device__ __forceinline__ h8_t k_load(uint32_t k, int u) const {
+    const int c = u / (PARTS * NKB), part = u / NKB % PARTS, kb = u % NKB;
+    return k_read<D>((k ^ 32 * c) + part * SIDE, kb);
+  }
+  __device__ __forceinline__ void k_mma(int u, const h8_t f, f16v_t* s) const {
+    const int c = u / (PARTS * NKB), part = u / NKB % PARTS, kb = u % NKB;
+    s[kb] = mma<BF>(f, q[c], s[kb]);
+    if constexpr (QLO) {
+      if (part == 0) s[kb] = mma<BF>(f, ql[c], s[kb]);
+    }
+  }
+  // Scores of the keys at LDS address k (k_at's lane offset included).
+  template <int SIDE>
+  __device__ __forceinline__ void scores(uint32_t k, f16v_t* s) const {
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) s[kb] = f16v_t{};
+    h8_t f[RING];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) f[u] = k_load<SIDE>(k, u);
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      if (u + AHEAD < UNITS) f[(u + AHEAD) % RING] = k_load<SIDE>(k, u + AHEAD);
+      k_mma(u, f[u % RING], s);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  __device__ __forceinline__ float top(const f16v_t* s) const {  // largest scaled score of the lane's column
+    float x = -kInf;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x = fmaxf(x, s[kb][i]);
+    return halves_max(x) * scale;
+  }
+  // The running maximum moves only when a row's passes it by more than 2^8: weights stay below
+  // 2^8 meanwhile.
+  __device__ __forceinline__ void rescale(float mt) {
+    if (__builtin_amdgcn_ballot_w64(mt > m + 8.f)) {
+      const float m_new = fmaxf(m, mt);
+      const float alpha = m_new == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
+      m = m_new;
+    }
+  }
+  // Scores to rounded weights (p[ks]: 16 keys), and with NEXT the next step's scores. Pair n's
+  // exponentials are one slot ahead of its sum and rounding.
+  template <bool NEXT, int SIDE>
+  __device__ __forceinline__ void weights(const f16v_t* s, u4_t* p, uint32_t k, f16v_t* next) {
+    const float ms = m == -kInf ? 0.f : m - kShift;
+    float sum[2] = {0.f, 0.f}, x[2][2];
+    auto ex = [&](int n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        x[n & 1][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n / 8][2 * (n % 8) + e], scale, -ms));
+    };
+    auto put = [&](int n) {
+      sum[0] += x[n & 1][0];
+      sum[1] += x[n & 1][1];
+      p[n / 4][n % 4] = pack2<BF>(x[n & 1][0], x[n & 1][1]);
+    };
+    if constexpr (NEXT) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) next[kb] = f16v_t{};
+      h8_t f[RING];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) f[u] = k_load<SIDE>(k, u);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        if (u + AHEAD < UNITS) f[(u + AHEAD) % RING] = k_load<SIDE>(k, u + AHEAD);
+        k_mma(u, f[u % RING], next);
+#pragma unroll
+        for (int n = u * (NP + 1) / UNITS; n < (u + 1) * (NP + 1) / UNITS; ++n) {
+          if (n < NP) ex(n);
+          if (n > 0) put(n - 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        ex(n);
+        put(n);
+      }
+    }
+    asm volatile("" : "+v"(sum[0]), "+v"(sum[1]));  // made here, not where l is used: 32 registers
+    l += sum[0] + sum[1];
+  }
+  // O^T += V^T P^T over the values at LDS address v (v_at's lane offset included); returns top() of
+  // `next`, taken along.
+  template <bool NEXT>
+  __device__ __forceinline__ float values(const u4_t* p, uint32_t v, const f16v_t* next) {
+    constexpr int VU = 2 * NKB * NDB;  // 16 keys x 32 channels each
+    auto load = [&](int u) { return v_read<D>(v ^ 64 * (u % NDB), u / NDB); };
+    h8_t f[RING];
+    float x = -kInf;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) f[u] = load(u);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < VU; ++u) {
+      if (u + AHEAD < VU) f[(u + AHEAD) % RING] = load(u + AHEAD);
+      acc[u % NDB] = mma<BF>(f[u % RING], __builtin_bit_cast(h8_t, p[u / NDB]), acc[u % NDB]);
+      if constexpr (NEXT) {
+#pragma unroll
+        for (int n = u * NP / VU; n < (u + 1) * NP / VU; ++n)
+          x = fmaxf(fmaxf(x, next[n / 8][2 * (n % 8)]), next[n / 8][2 * (n % 8) + 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return NEXT ? halves_max(x) * scale : 0.f;
+  }
+};
+
 typedef float f4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 
