@@ -660,12 +660,15 @@ bool prefix_mfma(const echokv_layout* L) {
          L->num_blocks * L->chunks_per_page < (1LL << 24);
 }
 
-// Ranges of a shared prefix: enough workgroups for the chip (two for each of its 256
-// CUs) with at least 128 keys each.
+// Ranges of a shared prefix, at least 128 keys each: as many as keep the workgroups within the
+// chip's 256 CUs (one each). A second round of them costs more than it fills: 594 rows of GQA 4
+// behind 2048 keys (80 workgroups a range) take 87, 74 and 94 us in 2, 3 and 4 ranges, 64 of
+// GQA 4 behind 4096 (8 a range) 74, 63 and 61 in 8, 16 and 32, 256 of GQA 4 behind 16384 (32)
+// 317, 206 and 225 in 4, 8 and 16, 8065 rows behind 8192 (1008) 2001 and 2222 in 1 and 2.
 int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
   const int64_t n_rows = n * (hq / L->num_kv_heads), rows = prefix_mfma(L) ? ek::prefix_rows(L->head_size, ECHOKV_F16, n_rows) : 64;
   const int64_t wgs = (n_rows + rows - 1) / rows * L->num_kv_heads;
-  int64_t r = ((rows == 256 ? 256 : 512) + wgs - 1) / wgs;
+  int64_t r = 256 / (wgs > 0 ? wgs : 1);
   const int64_t most = len / 128;
   r = r < most ? r : most;
   return (int)(r < 1 ? 1 : r < 64 ? r : 64);

@@ -287,72 +287,93 @@ __global__ __launch_bounds__(256) void prefix_any_kernel(PrefixArgs a) {
 }
 
 // One wave per (entry, query head): its prefix ranges, then its suffix splits, 64 pieces at a
-// time, the rows of 8 requested together. Lane l takes channels l, l + 64, ...
-template <int C>
+// time, a group of 8 rows requested while the one before is added (the kernel is a chain of
+// round trips to memory). Lane l holds channels [C l, C l + C) where the head is 64 C channels
+// (ANY false: one vector load a piece), else l, l + 64, ...
+template <int C, bool ANY>
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
+  constexpr int GROUP = 8;
+  typedef float vec_t __attribute__((ext_vector_type(C)));
   const int lane = threadIdx.x & 63;
   const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);  // entry * hq + head
   if (row >= a.n * a.hq) return;
-  const long t = row / a.hq;
-  const int qh = (int)(row % a.hq), D = a.D;
-  if (a.lens && a.lens[t] < a.len) return;
-  int pieces = a.ranges;
+  const int t = (int)((unsigned)row / (unsigned)a.hq), qh = (int)row - t * a.hq, D = a.D;
+  const long len = a.lens ? a.lens[t] : 0;
+  int count = a.ranges;
   if (a.acc) {
     const int nb = ((int)a.suffix[t] + a.BS - 1) / a.BS;
-    if (nb > 0) {
-      const int bps = split_blocks(a.sp, nb);
-      pieces += (nb + bps - 1) / bps;
-    }
+    const int bps = split_blocks(a.sp, nb);
+    count += nb > 0 ? (nb + bps - 1) / bps : 0;
   }
   // Piece i's row of its workspace.
-  auto at = [&](int i) { return i < a.ranges ? (long)i * a.n * a.hq + row : row * a.num_splits + (i - a.ranges); };
-  float m = -kInf, den = 0.f, o[C] = {};
-  for (int p0 = 0; p0 < pieces; p0 += 64) {
-    float2 x = float2{-kInf, 0.f};
-    if (p0 + lane < pieces) {
-      const int i = p0 + lane;
-      x = *(const float2*)((i < a.ranges ? a.p_ml : a.ml) + 2 * at(i));
+  const long stride = a.n * a.hq, split0 = row * a.num_splits - a.ranges;
+  auto at = [&](int i) { return i < a.ranges ? row + i * stride : split0 + i; };
+  auto load = [&](int i0, int last, float (*y)[C]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < GROUP; ++u) {
+      const int i = min(i0 + u, last);
+      const float* src = (i < a.ranges ? a.p_acc : a.acc) + at(i) * D;
+      if constexpr (ANY) {
+#pragma unroll
+        for (int e = 0; e < C; ++e) y[u][e] = src[min(lane + 64 * e, D - 1)];
+      } else {
+        const vec_t v = *(const vec_t*)(src + C * lane);
+#pragma unroll
+        for (int e = 0; e < C; ++e) y[u][e] = v[e];
+      }
     }
+  };
+  float m = -kInf, den = 0.f, o[C] = {};
+  for (int p0 = 0; p0 < count; p0 += 64) {
+    const int n = min(64, count - p0);
+    float y[2][GROUP][C];
+    float2 x = float2{-kInf, 0.f};
+    if (lane < n) x = *(const float2*)((p0 + lane < a.ranges ? a.p_ml : a.ml) + 2 * at(p0 + lane));
+    load(p0, p0 + n - 1, y[0]);
     float mt = x.x;
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) mt = fmaxf(mt, __shfl_xor(mt, k, 64));
     const float top = fmaxf(m, mt);
-    if (top == -kInf) continue;
+    const float alpha = top == -kInf ? 1.f : __builtin_amdgcn_exp2f(m - top);
     const float w = x.x == -kInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
     float d = w * x.y;
 #pragma unroll
     for (int k = 32; k > 0; k >>= 1) d += __shfl_xor(d, k, 64);
-    const float alpha = __builtin_amdgcn_exp2f(m - top);
     den = den * alpha + d;
 #pragma unroll
     for (int e = 0; e < C; ++e) o[e] *= alpha;
     m = top;
-    const int last = min(pieces, p0 + 64);
-    for (int i0 = p0; i0 < last; i0 += 8) {
-      float y[8][C];
+    auto add = [&](int i0, float (*z)[C]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = i0 + u < last ? i0 + u : p0;
-        const float* src = (i < a.ranges ? a.p_acc : a.acc) + at(i) * D;
+      for (int u = 0; u < GROUP; ++u) {
+        if (i0 + u >= n) continue;
+        const float wu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i0 + u));
+        if (wu == 0.f) continue;  // an empty piece, whatever its row holds
 #pragma unroll
-        for (int e = 0; e < C; ++e) y[u][e] = lane + 64 * e < D ? src[lane + 64 * e] : 0.f;
+        for (int e = 0; e < C; ++e) o[e] = __builtin_fmaf(wu, z[u][e], o[e]);
       }
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        if (i0 + u >= last) continue;
-        const float wu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), i0 + u - p0));
-        if (wu == 0.f) continue;  // an empty piece
-#pragma unroll
-        for (int e = 0; e < C; ++e) o[e] = __builtin_fmaf(wu, y[u][e], o[e]);
-      }
+    };
+    for (int i0 = 0; i0 < n; i0 += 2 * GROUP) {
+      if (i0 + GROUP < n) load(p0 + i0 + GROUP, p0 + n - 1, y[1]);
+      add(i0, y[0]);
+      if (i0 + 2 * GROUP < n) load(p0 + i0 + 2 * GROUP, p0 + n - 1, y[0]);
+      if (i0 + GROUP < n) add(i0 + GROUP, y[1]);
     }
   }
+  if (a.lens && len < a.len) return;
   const long q_row = a.q_rows ? a.q_rows[t] : t;
   const float inv = den == 0.f ? 0.f : 1.f / den;
   if (a.lse && lane == 0) a.lse[q_row * a.hq + qh] = den == 0.f ? -kInf : m + __log2f(den);
+  const long ob = q_row * a.o_s0 + (long)qh * a.o_s1;
+  if constexpr (ANY) {
 #pragma unroll
-  for (int e = 0; e < C; ++e)
-    if (lane + 64 * e < D) st(a.out, a.out_dtype, q_row * a.o_s0 + (long)qh * a.o_s1 + lane + 64 * e, o[e] * inv);
+    for (int e = 0; e < C; ++e)
+      if (lane + 64 * e < D) st(a.out, a.out_dtype, ob + lane + 64 * e, o[e] * inv);
+  } else {
+#pragma unroll
+    for (int e = 0; e < C; ++e) o[e] *= inv;
+    st_n<C>(a.out, a.out_dtype, ob + C * lane, o);
+  }
 }
 
 hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s) {
@@ -373,9 +394,11 @@ hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s) {
 
 hipError_t launch_join(const JoinArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.n * a.hq + 3) / 4));
-  if (a.D <= 64) hipLaunchKernelGGL(join_kernel<1>, grid, dim3(256), 0, s, a);
-  else if (a.D <= 128) hipLaunchKernelGGL(join_kernel<2>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(join_kernel<4>, grid, dim3(256), 0, s, a);
+  if (a.D == 64) hipLaunchKernelGGL((join_kernel<1, false>), grid, dim3(256), 0, s, a);
+  else if (a.D == 128) hipLaunchKernelGGL((join_kernel<2, false>), grid, dim3(256), 0, s, a);
+  else if (a.D == 256) hipLaunchKernelGGL((join_kernel<4, false>), grid, dim3(256), 0, s, a);
+  else if (a.D < 128) hipLaunchKernelGGL((join_kernel<2, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<4, true>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
