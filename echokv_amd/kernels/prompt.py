@@ -86,40 +86,56 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     (``kernels.shared.prefix_attention``), joined with the result."""
     if plan is None and not prefill:
         return
-    if query.dim() != 3 or key.dim() != 3 or value.shape != key.shape:
+    qs, ks = query.shape, key.shape
+    if len(qs) != 3 or len(ks) != 3 or value.shape != ks:
         raise ValueError("query must be [T, Hq, D], key and value [T, H, D]")
-    hq, h, d = query.shape[1], key.shape[1], query.shape[2]
-    if h == 0 or hq % h or key.shape[2] != d:
-        raise ValueError(f"{hq} query heads of {d} channels do not fit {h} KV heads of {key.shape[2]}")
-    if key.dtype != query.dtype or value.dtype != query.dtype:
-        raise ValueError(f"query, key and value must share a dtype, got {query.dtype}, {key.dtype}, {value.dtype}")
-    out = _out_view(output, hq)
-    if out.shape[1:] != query.shape[1:]:
-        raise ValueError(f"output rows of shape {tuple(out.shape[1:])}, the query's are {tuple(query.shape[1:])}")
-    _lib.require_current(query, key, value, output, lse)
+    t, hq, d = qs
+    h = ks[1]
+    if h == 0 or hq % h or ks[2] != d:
+        raise ValueError(f"{hq} query heads of {d} channels do not fit {h} KV heads of {ks[2]}")
+    dtype = query.dtype
+    if key.dtype != dtype or value.dtype != dtype:
+        raise ValueError(f"query, key and value must share a dtype, got {dtype}, {key.dtype}, {value.dtype}")
+    out = output if output.dim() == 3 else _out_view(output, hq)
+    out_rows, out_hq, out_d = out.shape
+    if out_hq != hq or out_d != d:
+        raise ValueError(f"output rows of shape {(out_hq, out_d)}, the query's are {(hq, d)}")
     if plan is None:
+        _lib.require_current(query)
         plan = build_prompt_plan(prefill, hq // h, d, query.device)
+    part, p_lse = prefix if prefix is not None else (None, None)
+    _lib.require_current(query, key, value, output, lse, part, p_lse, plan.tiles)
     if plan.gqa != hq // h or plan.head_size != d:
         raise ValueError("the plan was built for other heads")
-    if plan.rows > min(t.shape[0] for t in (query, key, value, out)):
+    if plan.rows > min(t, ks[0], out_rows):
         raise ValueError(f"the prompts reach row {plan.rows}, the tensors hold fewer")
-    if plan.tiles.shape[0] == 0:
+    n_tiles = plan.tiles.shape[0]
+    if n_tiles == 0:
         return
-    _lib.require_current(plan.tiles)
-    query, key, value = (t if t.stride(2) == 1 else t.contiguous() for t in (query, key, value))
+    (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(query), _rows(key), _rows(value)
+    o0, o1, o2 = out.stride()
+    if o2 != 1:
+        raise ValueError("output rows must be contiguous along head_dim")
+    p0 = p1 = 0
     if lse is not None:
         _row_state(lse, plan.rows, hq, "lse")
-    part, p_lse, p_s = None, None, (0, 0)
-    if prefix is not None:
-        part, p_lse = prefix
-        _lib.require_current(part, p_lse)
-        if part.dtype != torch.float32 or part.shape[1:] != query.shape[1:] or part.shape[0] < plan.rows or part.stride(2) != 1:
+    if part is not None:
+        if part.dtype != torch.float32 or part.shape[1:] != qs[1:] or part.shape[0] < plan.rows or part.stride(2) != 1:
             raise ValueError("prefix rows must be float32 [T, Hq, D] with contiguous channels")
         _row_state(p_lse, plan.rows, hq, "the prefix's log-sum-exp")
-        p_s = part.stride(0), part.stride(1)
+        p0, p1, _ = part.stride()
+    code = _lib.dtype_code(query)
     _lib.call(
-        "echokv_prompt", _lib.ptr(query), query.stride(0), query.stride(1), _lib.ptr(key), key.stride(0), key.stride(1),
-        _lib.ptr(value), value.stride(0), value.stride(1), _lib.dtype_code(query), hq, h, d, _lib.ptr(plan.tiles),
-        plan.tiles.shape[0], plan.tile_m, float(softmax_scale), _lib.ptr(part), *p_s, _lib.ptr(p_lse), _lib.ptr(out),
-        out.stride(0), out.stride(1), _lib.dtype_code(out), _lib.ptr(lse), _lib.stream(),
+        "echokv_prompt", q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, code, hq, h, d,
+        plan.tiles.data_ptr(), n_tiles, plan.tile_m, float(softmax_scale), _lib.ptr(part), p0, p1, _lib.ptr(p_lse),
+        out.data_ptr(), o0, o1, code if out.dtype == dtype else _lib.dtype_code(out), _lib.ptr(lse), _lib.stream(),
     )
+
+
+def _rows(t: torch.Tensor) -> tuple:
+    """``t`` with contiguous channels, and its row and head strides."""
+    s0, s1, s2 = t.stride()
+    if s2 != 1:
+        t = t.contiguous()
+        s0, s1, _ = t.stride()
+    return t, s0, s1

@@ -23,9 +23,9 @@ from echokv_amd.kernels import decode as dec
 
 
 def _query(store, query: torch.Tensor) -> torch.Tensor:
-    L = store.layout
-    if query.dim() != 3 or query.shape[2] != L.head_size or query.shape[1] == 0 or query.shape[1] % L.num_kv_heads:
-        raise ValueError(f"query of shape {tuple(query.shape)} does not fit {L.num_kv_heads} KV heads of {L.head_size}")
+    L, shape = store.layout, query.shape
+    if len(shape) != 3 or shape[2] != L.head_size or shape[1] == 0 or shape[1] % L.num_kv_heads:
+        raise ValueError(f"query of shape {tuple(shape)} does not fit {L.num_kv_heads} KV heads of {L.head_size}")
     return query if query.stride(2) == 1 else query.contiguous()
 
 
@@ -37,9 +37,9 @@ def _blocks(store, blocks: torch.Tensor, prefix_len: int) -> torch.Tensor:
     return blocks if blocks.dtype == torch.int32 and blocks.stride(0) == 1 else blocks.to(torch.int32).contiguous()
 
 
-def _workspace(workspace: torch.Tensor | None, need: int, device) -> torch.Tensor:
+def _workspace(workspace: torch.Tensor | None, need: int, device) -> torch.Tensor | None:
     if workspace is None:
-        return torch.empty(max(need, 1), dtype=torch.uint8, device=device)
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
     if workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.numel() < need:
         raise ValueError(f"the workspace must be {need} contiguous uint8 bytes")
     if workspace.data_ptr() % 16:
@@ -73,11 +73,13 @@ def prefix_attention(store, query: torch.Tensor, blocks: torch.Tensor, prefix_le
         raise ValueError(f"lse must be contiguous float32 {(t, hq)}")
     ws = _workspace(workspace, need, query.device)
     res = _lib.residual(store.res_k)
+    q0, q1, _ = query.stride()
+    p0, p1, _ = part.stride()
     _lib.call(
-        "echokv_prefix", _lib.byref(store.abi), _lib.ptr(store.pages), _lib.ptr(store.block_res),
-        _lib.ptr(store.res_group), _lib.byref(res), _lib.ptr(query), query.stride(0), query.stride(1),
-        _lib.dtype_code(query), hq, None, t, _lib.ptr(blocks), prefix_len, float(softmax_scale), _lib.ptr(ws),
-        ws.numel(), _lib.ptr(part), part.stride(0), part.stride(1), _lib.ptr(lse), _lib.stream(),
+        "echokv_prefix", _lib.byref(store.abi), store.pages.data_ptr(), store.block_res.data_ptr(),
+        store.res_group.data_ptr(), _lib.byref(res), query.data_ptr(), q0, q1, _lib.dtype_code(query), hq, None, t,
+        blocks.data_ptr(), prefix_len, float(softmax_scale), _lib.ptr(ws), 0 if ws is None else ws.numel(),
+        part.data_ptr(), p0, p1, lse.data_ptr(), _lib.stream(),
     )
     return part, lse
 
@@ -140,7 +142,7 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
         num_splits = suffix_splits(block_table, L.block_size, prefix_len, blocks_per_split, max_len)
     need = shared_workspace_bytes(store, hq, s, prefix_len, int(num_splits))
     dev = query.device
-    lens, q_rows, bt_rows = (dec._i64(t, dev) for t in (seq_lens, q_rows, bt_rows))
+    lens, q_rows, bt_rows = dec._i64(seq_lens, dev), dec._i64(q_rows, dev), dec._i64(bt_rows, dev)
     if out is None:
         out = torch.empty(s if q_rows is None else query.shape[0], hq, d, device=dev, dtype=torch.float32)
     if out.dim() != 3 or out.shape[1:] != query.shape[1:] or out.stride(2) != 1:
@@ -153,12 +155,13 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
         tier = store.pool.majority_tier()
     ws = _workspace(workspace, need, dev)
     res = _lib.residual(store.res_k)
+    q0, q1, _ = query.stride()
+    o0, o1, _ = out.stride()
     _lib.call(
-        "echokv_shared_decode", _lib.byref(store.abi), _lib.ptr(store.pages), _lib.ptr(store.block_res),
-        _lib.ptr(store.res_group), _lib.byref(res), _lib.ptr(query), query.stride(0), query.stride(1),
-        _lib.dtype_code(query), hq, _lib.ptr(q_rows), _lib.ptr(block_table), block_table.stride(0), _lib.ptr(bt_rows),
-        _lib.ptr(lens), s, _lib.ptr(blocks), prefix_len, float(softmax_scale), int(num_splits), int(blocks_per_split),
-        int(tier), _lib.ptr(tier_mask), _lib.ptr(ws), ws.numel(), _lib.ptr(out), out.stride(0), out.stride(1),
-        _lib.dtype_code(out), _lib.stream(),
+        "echokv_shared_decode", _lib.byref(store.abi), store.pages.data_ptr(), store.block_res.data_ptr(),
+        store.res_group.data_ptr(), _lib.byref(res), query.data_ptr(), q0, q1, _lib.dtype_code(query), hq,
+        _lib.ptr(q_rows), block_table.data_ptr(), block_table.stride(0), _lib.ptr(bt_rows), lens.data_ptr(), s,
+        blocks.data_ptr(), prefix_len, float(softmax_scale), int(num_splits), int(blocks_per_split), int(tier),
+        _lib.ptr(tier_mask), ws.data_ptr(), ws.numel(), out.data_ptr(), o0, o1, _lib.dtype_code(out), _lib.stream(),
     )
     return out
