@@ -56,6 +56,8 @@ from echokv_amd.controller import SUPPORTED_BITS, LayerController
 from echokv_amd.host_slots import host_lens_and_slots, is_dummy_step
 from echokv_amd.kernels import decode as dec
 from echokv_amd.kernels import prefill as pf
+from echokv_amd.kernels import prompt as pm
+from echokv_amd.kernels import shared as sh
 from echokv_amd.step import StepDriver
 from echokv_amd.tiered_cache import HeaderWriter, TieredKVCache, TieredLayout
 from echokv_amd.write_plan import SharedState, WriteMeta
@@ -67,6 +69,11 @@ KERNEL_HEAD_SIZES = (64, 128, 256)
 MAX_HEAD_SIZE = 256
 # Upper bound on decode splits per sequence (a fixed grid, so a graph replays it).
 MAX_DECODE_SPLITS = dec.MAX_SPLITS
+# A shared prefix from this long on is attended to apart (ECHOKV_SHARED_PREFIX=1). Apart it costs
+# two launches more, and its keys are a chain of steps in either form: decode of 1 to 64 requests
+# of 100-400 tokens behind 512 takes 27-36 us plainly, 32-42 apart; behind 1024 40-58 and 33-44;
+# behind 8192 73-193 and 40-61 (INT4, 8 KV heads of GQA 4 or 2 of GQA 8).
+SHARED_PREFIX_TOKENS = 1024
 
 
 class EchoKVAttentionBackend(AttentionBackend):
@@ -125,6 +132,16 @@ def block_multiple() -> int:
 # ---- per-step device work --------------------------------------------------------
 
 @dataclass
+class SharedPrefix:
+    """Cached blocks that every request of the step begins with."""
+
+    tokens: int  # a multiple of the block size
+    blocks: torch.Tensor  # int32 block list
+    num_splits: int = 0  # decode: splits of the tokens behind it
+    workspace: torch.Tensor | None = None  # decode: shared by every layer of the step
+
+
+@dataclass
 class DecodeWork:
     """One decode entry per single-token request (graph padding: length 0)."""
 
@@ -136,6 +153,7 @@ class DecodeWork:
     batch_invariant: bool
     tier_masks: torch.Tensor | None = None  # [layers, 2] int32: each layer's live tiers, read by the kernels
     host_tier_masks: np.ndarray | None = None  # [layers] the same, on the host
+    prefix: SharedPrefix | None = None  # cached blocks that every entry begins with, read once
 
     def run(self, impl, query: torch.Tensor, block_table: torch.Tensor, out: torch.Tensor) -> None:
         # Each tier the layer holds runs on its own fast path (tier passes, on the
@@ -145,6 +163,8 @@ class DecodeWork:
         # takes the tier passes on either schedule (the balanced kernel has none: its
         # other tiers' blocks would take the generic path, about 2.6x slower a block).
         tier, mask, inv, ws = impl.decode_tier(), None, self.batch_invariant, self.workspace
+        if self.prefix is not None:
+            inv = True  # the tokens behind the prefix run on the split schedule
         if self.tier_masks is not None:
             if _capturing(query):
                 if inv:
@@ -158,6 +178,12 @@ class DecodeWork:
                         ws = impl.split_workspace(ws, self.lens.shape[0], self.num_splits)
                 elif held:
                     tier = held
+        if self.prefix is not None:
+            p = self.prefix
+            sh.shared_prefix_decode(impl.store, query, block_table, self.lens, p.tokens, impl.scale, q_rows=self.rows,
+                                    bt_rows=self.reqs, blocks=p.blocks, out=out, num_splits=p.num_splits,
+                                    workspace=p.workspace, tier=tier, tier_mask=mask)
+            return
         dec.decode_attention(impl.store, query, block_table, self.lens, impl.scale, q_rows=self.rows,
                              bt_rows=self.reqs, out=out, num_splits=self.num_splits, workspace=ws,
                              tier=tier, batch_invariant=inv, tier_mask=mask)
@@ -172,15 +198,37 @@ class PrefillWork:
     tiles: torch.Tensor | None = None  # fused path (every chunk <= 64 tokens)
     dense: tuple | None = None  # (DensePlan, workspace) of the two-pass path
     own_group_rows: torch.Tensor | None = None  # own-group-exact prefill (ECHOKV_OWN_GROUP_EXACT=1)
+    prompts: list | None = None  # [PromptWork]: chunks that read this step's keys (ECHOKV_PROMPT_EXACT=1)
 
-    def run(self, impl, query: torch.Tensor, key: torch.Tensor, block_table: torch.Tensor,
+    def run(self, impl, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, block_table: torch.Tensor,
             out: torch.Tensor) -> None:
+        for work in self.prompts or ():
+            work.run(impl, query, key, value, out)
         og_key = None
         if self.own_group_rows is not None:  # each query's own K group from this step's key rows
             og_key = key.view(key.shape[0], impl.num_kv_heads, impl.head_size)
         pf.prefill_attention(impl.store, query, out, self.entries, self.reqs, block_table, impl.scale,
                              tiles=self.tiles, dense=self.dense, own_group_key=og_key,
                              own_group_rows=self.own_group_rows)
+
+
+@dataclass
+class PromptWork:
+    """Chunks that are whole prompts, or all of a prompt behind the shared prefix: they attend to
+    this step's keys and values, and to the prefix in the cache."""
+
+    rows: tuple  # the step's query rows [first, last) that hold them
+    plan: pm.PromptPlan  # of the chunks, by rows from the first one on
+    prefix: SharedPrefix | None = None
+
+    def run(self, impl, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, out: torch.Tensor) -> None:
+        a, b = self.rows
+        q, o = query[a:b], out[a:b]
+        k, v = (x.view(x.shape[0], impl.num_kv_heads, impl.head_size)[a:b] for x in (key, value))
+        before = None
+        if self.prefix is not None:
+            before = sh.prefix_attention(impl.store, q, self.prefix.blocks, self.prefix.tokens, impl.scale)
+        pm.prompt_attention(q, k, v, o, (), impl.scale, plan=self.plan, prefix=before)
 
 
 @dataclass
@@ -310,9 +358,14 @@ class EchoKVMetadataBuilder(AttentionMetadataBuilder):
         return self.group
 
     # -- the step ---------------------------------------------------------------
+    def use_cascade_attention(self, common_prefix_len: int, query_lens, *args, **kwargs) -> bool:
+        """vLLM asks before a step whether the requests' common prefix (cached blocks, in tokens) is
+        attended to apart; its length then reaches ``build`` (and the step runs outside full graphs)."""
+        return bool(self.cfg.shared_prefix and len(query_lens) > 1 and common_prefix_len >= SHARED_PREFIX_TOKENS)
+
     def build(self, common_prefix_len: int, common_attn_metadata, fast_build: bool = False) -> EchoKVMetadata:
         with record_function("echokv.build"):
-            return self._build(common_attn_metadata)
+            return self._build(common_attn_metadata, int(common_prefix_len))
 
     def _mapping(self, cm, dummy: bool):
         """The step's (lengths, slots) on the host: derived from host copies when vLLM
@@ -331,7 +384,22 @@ class EchoKVMetadataBuilder(AttentionMetadataBuilder):
             raise AssertionError("EchoKV host slot mapping differs from vLLM's")
         return dev
 
-    def _build(self, cm) -> EchoKVMetadata:
+    def _shared(self, cm, lens: torch.Tensor, qsl: np.ndarray, common_prefix_len: int) -> SharedPrefix | None:
+        """The step's shared prefix: whole blocks, before every request's first query token."""
+        if not self.cfg.shared_prefix or common_prefix_len <= 0:
+            return None
+        q_lens = qsl[1:] - qsl[:-1]
+        live = np.nonzero((q_lens > 0) & (lens.numpy() > 0))[0]
+        if not live.size:
+            return None
+        bs = self.kv_cache_spec.block_size
+        cached = int((lens.numpy()[live] - q_lens[live]).min())
+        tokens = min(common_prefix_len, cached) // bs * bs
+        if tokens < SHARED_PREFIX_TOKENS:
+            return None
+        return SharedPrefix(tokens, cm.block_table_tensor[int(live[0]), : tokens // bs].to(torch.int32).contiguous())
+
+    def _build(self, cm, common_prefix_len: int = 0) -> EchoKVMetadata:
         if getattr(cm, "causal", True) is not True:
             raise NotImplementedError("EchoKV supports causal decoder attention only")
         n, t = cm.num_reqs, cm.num_actual_tokens
@@ -347,6 +415,7 @@ class EchoKVMetadataBuilder(AttentionMetadataBuilder):
             self._score_canary(group)  # before this step's writes move the K_ref ring
         fire = self.canary.tick(dummy)
         qsl = np.ascontiguousarray(cm.query_start_loc_cpu[: n + 1].numpy(), dtype=np.int32)
+        prefix = None if dummy else self._shared(cm, lens, qsl, common_prefix_len)
         up = group.driver.run(qsl, np.ascontiguousarray(lens.numpy(), dtype=np.int32),
                               np.ascontiguousarray(slots.numpy(), dtype=np.int64), group.tiers(), fire)
         self.canary.fired(up.n_canary, up.canary_ctx)
@@ -360,13 +429,42 @@ class EchoKVMetadataBuilder(AttentionMetadataBuilder):
                                    host_tier_masks=up.host_tier_masks,
                                    workspace=group.impls[0].decode_workspace(n_dec, self.num_splits, self.cap),
                                    batch_invariant=self.cfg.batch_invariant)
+            if prefix is not None:
+                md.decode.prefix = self._decode_prefix(group, prefix, n_dec, int(lens.max()))
         if up.prefill:
-            md.prefill = self._prefill_work(group, up.prefill)
+            md.prefill = self._prefill_work(group, up.prefill, prefix)
         return md
 
-    def _prefill_work(self, group: _Group, chunks: list) -> PrefillWork:
+    def _decode_prefix(self, group: _Group, prefix: SharedPrefix, n_dec: int, longest: int) -> SharedPrefix:
+        """``prefix`` with the splits and the workspace of the step's decode."""
+        store, hq = group.impls[0].store, group.impls[0].num_heads
+        bs = self.kv_cache_spec.block_size
+        splits = sh.suffix_splits(-(-longest // bs), bs, prefix.tokens, dec.BLOCKS_PER_SPLIT, longest)
+        need = sh.shared_workspace_bytes(store, hq, n_dec, prefix.tokens, splits)
+        return replace(prefix, num_splits=splits, workspace=torch.empty(need, dtype=torch.uint8, device=self.device))
+
+    def _prompt_work(self, chunks: list, prefix: SharedPrefix | None) -> tuple[list, list]:
+        """(the chunks that read this step's keys as ``PromptWork``, the other chunks)."""
+        head_size = self.kv_cache_spec.head_size
+        work = []
+        shared = prefix.tokens if prefix is not None else 0
+        for before in dict.fromkeys((0, shared)):
+            mine = [(qs, qe) for qs, qe, ctx, _ in chunks if ctx - (qe - qs) == before]
+            if mine:
+                first, last = min(a for a, _ in mine), max(b for _, b in mine)
+                plan = pm.build_prompt_plan([(a - first, b - first) for a, b in mine], self.gqa, head_size, self.device)
+                work.append(PromptWork((first, last), plan, prefix if before else None))
+        rest = [c for c in chunks if c[2] - (c[1] - c[0]) not in (0, shared)]
+        return work, rest
+
+    def _prefill_work(self, group: _Group, chunks: list, prefix: SharedPrefix | None = None) -> PrefillWork:
+        prompts = None
+        if self.cfg.prompt_exact:
+            prompts, chunks = self._prompt_work(chunks, prefix)
+            if not chunks:
+                return PrefillWork(entries=[], reqs=[], prompts=prompts)
         entries = [(qs, qe, ctx, 0) for qs, qe, ctx, _ in chunks]
-        work = PrefillWork(entries=entries, reqs=[r for *_, r in chunks])
+        work = PrefillWork(entries=entries, reqs=[r for *_, r in chunks], prompts=prompts)
         impl0 = group.impls[0]
         dev = self.device
         if pf.kernels_take(impl0.head_size, self.gqa):
@@ -540,7 +638,7 @@ class EchoKVAttentionImpl(AttentionImpl):
         out = output.view(output.shape[0], -1, query.shape[-1])
         if md.prefill is not None:
             with record_function("echokv.prefill_attn"):
-                md.prefill.run(self, query, key, md.block_table, out)
+                md.prefill.run(self, query, key, value, md.block_table, out)
         if md.decode is not None:
             with record_function("echokv.decode_attn"):
                 md.decode.run(self, query, md.block_table, out)

@@ -22,15 +22,17 @@ raises are those of ``echokv_vllm/config.py:40-99``:
     ECHOKV_CANARY_MAX_Q     decode queries sampled per fire (default 8)
 
 This build's own: ECHOKV_OWN_GROUP_EXACT=1 (prefill sees each query's own K
-group at full precision) and ECHOKV_BATCH_INVARIANT=0 (the balanced decode
-schedule); ECHOKV_V_GROUP is 1 to 256 channels.
+group at full precision), ECHOKV_BATCH_INVARIANT=0 (the balanced decode
+schedule), ECHOKV_PROMPT_EXACT=1 (whole prompts attend to their own keys and values at
+full precision) and ECHOKV_SHARED_PREFIX=1 (a prefix that the batch shares is read once);
+ECHOKV_V_GROUP is 1 to 256 channels.
 
 Read elsewhere: ECHOKV_CUDAGRAPH=0 keeps attention out of full graphs (the
 backend), ECHOKV_CHECK_HOST_SLOTS=1 checks the host slot mapping every step. The
 reference's Triton-only switches (ECHOKV_DISABLE_TRITON, ECHOKV_AUTOTUNE,
 ECHOKV_PREFILL_ROWS) have no meaning here and are ignored.
 
-Each setting is one row of ``SETTINGS``: its variable, how to parse it, its
+Each setting is one row of ``SETTINGS`` or ``ATTENTION_SETTINGS``: its variable, how to parse it, its
 default (a function of the settings resolved before it) and its check. Rows are
 resolved in order, then checked in order, so the first bad value raises.
 """
@@ -55,6 +57,8 @@ class EchoKVConfig:
     canary_max_q: int = 8
     own_group_exact: bool = False
     batch_invariant: bool = True
+    prompt_exact: bool = False
+    shared_prefix: bool = False
     controller: ControllerParams = field(default_factory=ControllerParams)
 
 
@@ -129,6 +133,17 @@ SETTINGS: tuple[Setting, ...] = (
     Setting("ECHOKV_BATCH_INVARIANT", "batch_invariant", lambda raw: raw != "0", lambda s: True),
 )
 
+# Attention paths beside the reference's, this build's own.
+ATTENTION_SETTINGS: tuple[Setting, ...] = (
+    # Prompts without cached context (or, with the next setting, behind the shared prefix)
+    # attend to this step's keys and values instead of reading them back quantized from the cache.
+    Setting("ECHOKV_PROMPT_EXACT", "prompt_exact", _flag, lambda s: False),
+    # Cached blocks that every request of a step begins with are attended to once for the batch
+    # (vLLM's cascade attention); a request's result then depends on its batch through float
+    # rounding.
+    Setting("ECHOKV_SHARED_PREFIX", "shared_prefix", _flag, lambda s: False),
+)
+
 _CONTROLLER_KEYS = ("tau0", "l0", "tau_scaling", "alpha", "init_bits", "fixed_bits", "frozen")
 
 
@@ -136,10 +151,11 @@ def resolve(environ=None) -> dict:
     """Every setting's value (parsed, or its default), after all checks pass."""
     env = os.environ if environ is None else environ
     vals: dict = {}
-    for st in SETTINGS:
+    table = SETTINGS + ATTENTION_SETTINGS
+    for st in table:
         raw = env.get(st.env)
         vals[st.key] = st.default(vals) if raw is None or raw == "" else st.parse(raw)
-    for st in SETTINGS:
+    for st in table:
         if st.check is not None and (msg := st.check(vals[st.key], vals)):
             raise ValueError(msg)
     return vals

@@ -95,10 +95,11 @@ def shared_workspace_bytes(store, num_q_heads: int, num_seqs: int, prefix_len: i
                      num_splits)
 
 
-def suffix_splits(block_table: torch.Tensor, block_size: int, prefix_len: int, blocks_per_split: int,
+def suffix_splits(max_blocks: int, block_size: int, prefix_len: int, blocks_per_split: int,
                   max_len: int | None) -> int:
-    """Splits of the tokens behind the prefix when the caller names none."""
-    cols = max(0, block_table.shape[1] - prefix_len // block_size)
+    """Splits of the tokens behind the prefix for sequences of at most ``max_blocks`` blocks (and
+    ``max_len`` tokens)."""
+    cols = max(0, max_blocks - prefix_len // block_size)
     longest = cols if max_len is None else min(cols, -(-max(0, max_len - prefix_len) // block_size))
     return max(dec.SHORT_SPLITS, min(-(-longest // blocks_per_split), dec.MAX_SPLITS))
 
@@ -139,7 +140,7 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
     if s and blocks is None and block_table.shape[0] == 0:
         raise ValueError("the block table has no row to take the shared blocks from")
     if num_splits is None:
-        num_splits = suffix_splits(block_table, L.block_size, prefix_len, blocks_per_split, max_len)
+        num_splits = suffix_splits(block_table.shape[1], L.block_size, prefix_len, blocks_per_split, max_len)
     need = shared_workspace_bytes(store, hq, s, prefix_len, int(num_splits))
     dev = query.device
     lens, q_rows, bt_rows = dec._i64(seq_lens, dev), dec._i64(q_rows, dev), dec._i64(bt_rows, dev)

@@ -149,5 +149,75 @@ def test_shared_python_refusals(lib):
     assert sh._blocks(store, table[0], 49).numel() == 4
     with pytest.raises(ValueError):
         sh._workspace(torch.zeros(10, dtype=torch.uint8), 11, CPU)
-    assert sh.suffix_splits(table, 16, 64, 16, None) == 4
-    assert sh.suffix_splits(torch.zeros(1, 4096), 16, 64, 16, None) == 64
+    assert sh.suffix_splits(8, 16, 64, 16, None) == 4
+    assert sh.suffix_splits(4096, 16, 64, 16, None) == 64
+
+
+# ---- the backend's side ----------------------------------------------------------------
+
+def _builder(monkeypatch, **env):
+    from echokv_amd.backend import EchoKVMetadataBuilder
+
+    for k, v in env.items():
+        monkeypatch.setenv(k, v)
+    cfg = SimpleNamespace(model_config=SimpleNamespace(max_model_len=4096, dtype=torch.float16,
+                                                       get_num_attention_heads=lambda pc: 8),
+                          parallel_config=None, scheduler_config=SimpleNamespace(max_num_seqs=8),
+                          compilation_config=SimpleNamespace(max_cudagraph_capture_size=8), speculative_config=None)
+    spec = SimpleNamespace(block_size=64, num_kv_heads=2, head_size=128)
+    return EchoKVMetadataBuilder(spec, ["l"], cfg, CPU)
+
+
+def test_settings_are_off_by_default(monkeypatch):
+    from echokv_amd.config import load_config
+
+    for k in ("ECHOKV_PROMPT_EXACT", "ECHOKV_SHARED_PREFIX"):
+        monkeypatch.delenv(k, raising=False)
+    cfg = load_config()
+    assert not cfg.prompt_exact and not cfg.shared_prefix
+    assert load_config({"ECHOKV_PROMPT_EXACT": "1"}).prompt_exact
+    assert load_config({"ECHOKV_SHARED_PREFIX": "1"}).shared_prefix
+    b = _builder(monkeypatch)
+    assert not b.use_cascade_attention(8192, [1, 1, 1], 8, 2, False, False, False, 256)
+
+
+def test_cascade_is_taken_from_the_measured_length_on(monkeypatch):
+    b = _builder(monkeypatch, ECHOKV_SHARED_PREFIX="1")
+    assert b.use_cascade_attention(1024, [1, 1], 8, 2, False, False, False, 256, dcp_world_size=1)
+    assert not b.use_cascade_attention(960, [1, 1], 8, 2)
+    assert not b.use_cascade_attention(4096, [1], 8, 2)
+
+
+def test_shared_prefix_of_a_step(monkeypatch):
+    """Whole blocks, before every live request's first query token; padding rows do not count."""
+    import numpy as np
+
+    b = _builder(monkeypatch, ECHOKV_SHARED_PREFIX="1")
+    table = torch.arange(4 * 40).view(4, 40)
+    cm = SimpleNamespace(block_table_tensor=table)
+
+    def of(starts, lens, common):
+        return b._shared(cm, torch.tensor(lens), np.array(starts, np.int32), common)
+
+    p = of([0, 0, 1, 8], [0, 2000, 1500], 1100)  # row 0 is padding
+    assert p.tokens == 1088 and p.blocks.tolist() == list(range(40, 57)) and p.blocks.dtype == torch.int32
+    assert of([0, 1, 11], [2000, 1098], 1088).tokens == 1088
+    assert of([0, 1, 11], [2000, 1097], 1088).tokens == 1024  # 1087 cached: 16 whole blocks
+    assert of([0, 1, 11], [2000, 1033], 1088) is None  # 1023 cached: 15, below the measured length
+    assert of([0, 1, 11], [2000, 1100], 0) is None
+    assert of([0, 0], [0], 2048) is None
+    assert _builder(monkeypatch, ECHOKV_SHARED_PREFIX="0")._shared(cm, torch.tensor([2000]), np.array([0, 1]), 1088) is None
+
+
+def test_prompt_chunks_are_told_apart(lib, monkeypatch):
+    from echokv_amd.backend import SharedPrefix
+
+    b = _builder(monkeypatch, ECHOKV_SHARED_PREFIX="1", ECHOKV_PROMPT_EXACT="1")
+    prefix = SharedPrefix(1088, torch.zeros(17, dtype=torch.int32))
+    chunks = [(3, 8, 5, 1), (8, 20, 1100, 2), (20, 30, 10, 3), (30, 40, 700, 4), (40, 41, 1089, 5)]
+    work, rest = b._prompt_work(chunks, prefix)
+    assert rest == [chunks[3]]
+    assert [(w.rows, w.plan.entries, w.prefix is prefix) for w in work] == [
+        ((3, 30), ((0, 5), (17, 27)), False), ((8, 41), ((0, 12), (32, 33)), True)]
+    work, rest = b._prompt_work(chunks, None)
+    assert len(work) == 1 and rest == [chunks[1], chunks[3], chunks[4]]
