@@ -143,7 +143,7 @@ __device__ __forceinline__ void load_q(const void* q, int dtype, long at, int D,
 
 // One workgroup per (tile, 64 of its rows, KV head); heads fastest.
 template <int DP>
-__global__ __launch_bounds__(256) void prompt_any_kernel(PromptArgs a) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_any_kernel(PromptArgs a) {
   using S = Steps<DP>;
   __shared__ __attribute__((aligned(16))) float kt[S::KEYS * S::PITCH], vt[S::KEYS * S::PITCH];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, c = lane >> 4;
@@ -163,22 +163,34 @@ __global__ __launch_bounds__(256) void prompt_any_kernel(PromptArgs a) {
   load_q<DP>(a.q, a.dtype, (row0 + tok) * a.q_s0 + (long)qh * a.q_s1, a.D, a.scale_log2, c, q);
   State<DP> st;
   st.init();
+  // A step's rows are requested while the one before is computed.
+  constexpr int ITEMS = S::KEYS * (DP / 4), NI = (ITEMS + 255) / 256;
+  float x[NI][4], y[NI][4];
+  auto fetch = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int i = tid + 256 * u, key = kb + i / (DP / 4), ch = 4 * (i % (DP / 4));
+      const long row = row0 + min(key, kv_end - 1);
+      const int c4 = ch < a.D ? ch : 0;
+      ld4(a.k, a.dtype, row * a.k_s0 + (long)h * a.k_s1 + c4, x[u]);
+      ld4(a.v, a.dtype, row * a.v_s0 + (long)h * a.v_s1 + c4, y[u]);
+    }
+  };
+  fetch(0);
   for (int kb = 0; kb < kv_end; kb += S::KEYS) {
     __syncthreads();
     bool odd = false;
-    for (int i = tid; i < S::KEYS * (DP / 4); i += 256) {
-      const int key = i / (DP / 4), ch = 4 * (i % (DP / 4));
-      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      if (kb + key < kv_end && ch < a.D) {
-        const long row = row0 + kb + key;
-        ld4(a.k, a.dtype, row * a.k_s0 + (long)h * a.k_s1 + ch, x);
-        ld4(a.v, a.dtype, row * a.v_s0 + (long)h * a.v_s1 + ch, y);
-        odd = odd || !finite4(y);
-      }
-      *(f4_t*)&kt[key * S::PITCH + ch] = f4_t{x[0], x[1], x[2], x[3]};
-      *(f4_t*)&vt[key * S::PITCH + ch] = f4_t{y[0], y[1], y[2], y[3]};
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int i = tid + 256 * u, key = i / (DP / 4), ch = 4 * (i % (DP / 4));
+      if (i >= ITEMS) break;
+      const bool there = kb + key < kv_end && ch < a.D;
+      odd = odd || (there && !finite4(y[u]));
+      *(f4_t*)&kt[key * S::PITCH + ch] = there ? f4_t{x[u][0], x[u][1], x[u][2], x[u][3]} : f4_t{0.f, 0.f, 0.f, 0.f};
+      *(f4_t*)&vt[key * S::PITCH + ch] = there ? f4_t{y[u][0], y[u][1], y[u][2], y[u][3]} : f4_t{0.f, 0.f, 0.f, 0.f};
     }
     const int any_odd = __syncthreads_or(odd);
+    if (kb + S::KEYS < kv_end) fetch(kb + S::KEYS);
     step_any<DP>(st, q, kt, vt, kb, lim, any_odd != 0, lane);
   }
   float l = st.l + __shfl_xor(st.l, 16, 64);
@@ -379,6 +391,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
 hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((long)a.n_tiles * a.H), (unsigned)(((long)a.tile_m * a.gqa + kRows - 1) / kRows));
   if (a.D <= 64) hipLaunchKernelGGL(prompt_any_kernel<64>, grid, dim3(256), 0, s, a);
+  else if (a.D <= 96) hipLaunchKernelGGL(prompt_any_kernel<96>, grid, dim3(256), 0, s, a);
   else if (a.D <= 128) hipLaunchKernelGGL(prompt_any_kernel<128>, grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL(prompt_any_kernel<256>, grid, dim3(256), 0, s, a);
   return hipGetLastError();
@@ -387,6 +400,7 @@ hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s) {
 hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.n * a.gqa + kRows - 1) / kRows * a.L.H * a.ranges));
   if (a.L.D <= 64) hipLaunchKernelGGL(prefix_any_kernel<64>, grid, dim3(256), 0, s, a);
+  else if (a.L.D <= 96) hipLaunchKernelGGL(prefix_any_kernel<96>, grid, dim3(256), 0, s, a);
   else if (a.L.D <= 128) hipLaunchKernelGGL(prefix_any_kernel<128>, grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL(prefix_any_kernel<256>, grid, dim3(256), 0, s, a);
   return hipGetLastError();
