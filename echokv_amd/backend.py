@@ -439,7 +439,7 @@ class EchoKVMetadataBuilder(AttentionMetadataBuilder):
         """``prefix`` with the splits and the workspace of the step's decode."""
         store, hq = group.impls[0].store, group.impls[0].num_heads
         bs = self.kv_cache_spec.block_size
-        splits = sh.suffix_splits(-(-longest // bs), bs, prefix.tokens, dec.BLOCKS_PER_SPLIT, longest)
+        splits = sh.suffix_splits(-(-longest // bs), bs, prefix.tokens, sh.suffix_blocks(store, n_dec), longest)
         need = sh.shared_workspace_bytes(store, hq, n_dec, prefix.tokens, splits)
         return replace(prefix, num_splits=splits, workspace=torch.empty(need, dtype=torch.uint8, device=self.device))
 

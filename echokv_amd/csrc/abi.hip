@@ -674,6 +674,16 @@ int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
   return (int)(r < 1 ? 1 : r < 64 ? r : 64);
 }
 
+// Whether the prefix is dequantized into a workspace first (16-bit queries, head size 64 or 128):
+// from three tiles of 256 rows on, and 8192 keys times tiles, less than which a second launch
+// takes longer than it saves. us in one pass / in two, GQA 4, 8 KV heads, INT4: 3 tiles over 1024
+// keys 26 / 29, over 4096 51 / 48, over 16384 124 / 115; 6 tiles 37 / 37, 77 / 65, 237 / 193;
+// 32 tiles 74 / 61, 272 / 212, 918 / 731; 2 tiles over 16384 keys 81 / 86.
+bool prefix_packed(const echokv_layout* L, int hq, int q_dtype, int64_t n, int64_t len) {
+  const int64_t tiles = (n * (hq / L->num_kv_heads) + 255) / 256;
+  return prefix_mfma(L) && L->head_size <= 128 && q_dtype != ECHOKV_F32 && tiles >= 3 && tiles * len >= 8192;
+}
+
 bool prefix_shape_ok(const echokv_layout* L, int hq, int64_t n, int64_t len) {
   if (!lay_ok(L) || L->head_size > ek::kMaxAnyD || hq <= 0 || hq % L->num_kv_heads) return false;
   // Grids: (rows / 64) x heads x ranges workgroups, rows / 4 waves of the join.
@@ -682,6 +692,11 @@ bool prefix_shape_ok(const echokv_layout* L, int hq, int64_t n, int64_t len) {
 
 // Float32 rows of `hq` heads and their (max, sum) pairs, behind one another.
 int64_t rows_bytes(int64_t rows, int D) { return rows * (D + 2) * 4; }
+
+// The dequantized prefix in front of them, where a call may use it (float32 queries do not).
+int64_t pack_bytes(const echokv_layout* L, int hq, int64_t n, int64_t len) {
+  return prefix_packed(L, hq, ECHOKV_F16, n, len) ? ek::prefix_pack_bytes(L->num_kv_heads, L->head_size, len) : 0;
+}
 
 // The shared part of echokv_prefix and echokv_shared_decode; n > 0 and the shapes checked.
 ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,
@@ -707,7 +722,9 @@ ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const i
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.ranges = ranges;
   a.per = (int)((len + ranges - 1) / ranges + 127) / 128 * 128;
-  a.acc = (float*)workspace;
+  const bool packed = prefix_packed(L, hq, q_dtype, n, len) && (uintptr_t)pages % 16 == 0;
+  a.pack = packed ? (uint8_t*)workspace : nullptr;
+  a.acc = (float*)((uint8_t*)workspace + pack_bytes(L, hq, n, len));
   a.ml = a.acc + ranges * n * hq * L->head_size;
   a.part = nullptr;
   a.p_s0 = a.p_s1 = 0;
@@ -733,7 +750,7 @@ int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int
   if (!prefix_shape_ok(L, num_q_heads, n, prefix_len)) return -ECHOKV_ESHAPE;
   if (n == 0) return 0;
   const int64_t ranges = prefix_ranges(L, num_q_heads, n, prefix_len);
-  return ranges > 1 ? rows_bytes(ranges * n * num_q_heads, L->head_size) : 0;
+  return pack_bytes(L, num_q_heads, n, prefix_len) + (ranges > 1 ? rows_bytes(ranges * n * num_q_heads, L->head_size) : 0);
 }
 
 int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res, const int64_t* res_group,
@@ -770,7 +787,8 @@ int64_t echokv_shared_decode_workspace(const echokv_layout* L, int32_t num_q_hea
   if (num_splits <= 0 || num_splits > (1 << 20)) return -ECHOKV_EINVAL;
   if (num_seqs == 0) return 0;
   const int64_t ranges = prefix_ranges(L, num_q_heads, num_seqs, prefix_len);
-  return (num_seqs * 8 + 15) / 16 * 16 + rows_bytes((ranges + num_splits) * num_seqs * num_q_heads, L->head_size);
+  return (num_seqs * 8 + 15) / 16 * 16 + pack_bytes(L, num_q_heads, num_seqs, prefix_len) +
+         rows_bytes((ranges + num_splits) * num_seqs * num_q_heads, L->head_size);
 }
 
 int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,
@@ -797,7 +815,7 @@ int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int
   a.lens = seq_lens;
   a.suffix = suffix;
   if (run_prefix(L, a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
-  float* acc = rows + ranges * num_seqs * num_q_heads * (L->head_size + 2);
+  float* acc = a.ml + ranges * num_seqs * num_q_heads * 2;
   float* ml = acc + num_splits * num_seqs * num_q_heads * L->head_size;
   ek::JoinArgs j{a.acc, a.ml, ranges, nullptr, nullptr, suffix, num_splits, ek::Splits{}, seq_lens, (int)prefix_len,
                  L->block_size, q_rows, num_seqs, num_q_heads, L->head_size, out, o_s0, o_s1, out_dtype, nullptr};

@@ -413,7 +413,10 @@ struct PrefixArgs {
   // (0: one chunk a page).
   int bs_shift, kg_shift;
   uint32_t kc_mul;
+  uint8_t* pack;  // nullable: the dequantized prefix, prefix_pack_bytes (16-bit queries, head size 64 or 128)
 };
+constexpr int kPackKeys = 64;  // keys of a tile of the dequantized prefix
+inline int64_t prefix_pack_bytes(int H, int D, int64_t len) { return (len + kPackKeys - 1) / kPackKeys * H * (kPackKeys * D * 6); }
 // Query rows of a workgroup of the 16-bit kernel: 32 per wave, four waves or (16-bit queries up to
 // head size 128, more than 128 rows) eight.
 inline int prefix_rows(int head_size, int q_dtype, int64_t rows) {

@@ -1,20 +1,27 @@
 // Attention of many query rows over one cached block list on 16-bit matrix instructions (head
 // sizes 64, 128 and 256, layouts whose items sit in one group; attend_any.hip takes the others).
 //
-// One workgroup per (128 query rows, KV head, range of keys): 32 rows per wave, rows are (entry, GQA
-// head) pairs, whatever sequence they belong to, so a key is dequantized once for 128 of them. A
-// step of 8192 / D keys is dequantized into LDS, keys as a float16 hi + lo pair (2^-22 of the
-// value together) and values in float16 (one rounding, as prefill.hip), and each wave runs S^T,
-// an online softmax and O^T over it (tiles.h). A thread dequantizes one item of a step (four keys
-// x eight channels of K and of V), its loads a chain spread over the steps: step i + 1's codes,
-// i + 2's page header and i + 3's block id are requested before step i's products.
+// One workgroup per (32 query rows per wave, KV head, range of keys): rows are (entry, GQA head)
+// pairs, whatever sequence they belong to, so a key is dequantized once for all of them. Keys are
+// held as a float16 hi + lo pair (2^-22 of the value together) and values in float16 (one
+// rounding, as prefill.hip); each wave runs S^T, an online softmax and O^T over a step's keys
+// (tiles.h).
+//
+// prefix_kernel dequantizes each step into LDS itself: a thread takes items of four keys x eight
+// channels, of K in the first four waves and of V in the others (four waves: of both), its loads a
+// chain spread over the steps (an item's codes are requested a step before they are needed, its
+// page header two and its block id three).
+//
+// With many rows the same keys would be dequantized again for every 256 of them:
+// prefix_pack_kernel dequantizes the prefix once into a workspace, in 64-key tiles laid out as
+// LDS holds them, and prefix_flash_kernel streams those by direct global-to-LDS loads, the loop of
+// prompt.hip.
 #include "items.h"
 #include "tiles.h"
 
 namespace ek {
 namespace {
 
-constexpr int kWaves = 4;
 constexpr float kInf = __builtin_inff();
 
 // An item's words: each row's eight codes in the 8 bytes at or before them.
@@ -26,66 +33,43 @@ struct Raw {
   bool ok;  // the item's keys can be read
 };
 
-}  // namespace
+struct Head {
+  uint4 h;
+  int blk, rs;  // rs: the low word (slots are small, -1: none)
+};
 
-template <int D, bool QLO, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) void prefix_kernel(PrefixArgs a) {
-  static_assert(WAVES == 4 || WAVES == 8, "a thread takes its items' K and V, or one of them");
-  constexpr bool BOTH = WAVES == 4;
-  constexpr int BUFS = BOTH ? 1 : 2;        // steps in LDS
-  constexpr int ROWS = 32 * WAVES;
-  constexpr int KEYS = 8192 / D;            // keys per step: 256 items
-  constexpr int NKB = KEYS >= 64 ? 2 : 1;   // 32-key blocks per softmax update
-  constexpr int NS = D / 16, NDB = D / 32, OCTS = D / 8;
-  constexpr int SIDE = KEYS * D * 2;        // bytes of K hi, then K lo, then V
-  constexpr float kShift = 6.f;             // weights are 2^6 times the softmax's: small ones keep their bits
-  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+// Items of the keys [k_begin, k_end) of head h in steps of KEYS: a thread's item of a step is four
+// keys x eight channels. Nothing loaded is looked at before the step that needs it, and no load
+// sits in a branch (addresses are clamped instead): the wave would wait for it there.
+template <int D, int KEYS>
+struct Items {
+  static constexpr int OCTS = D / 8, SIDE = KEYS * D * 2;  // bytes of a step's K hi, K lo or V
+  const PrefixArgs& a;
+  const int h, k_begin, k_end, oct, quad;
 
-  const Lay& L = a.L;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int tid = threadIdx.x, j = lane & 31, hh = lane >> 5;
-  if (a.suffix)
-    for (int t = (int)blockIdx.x * 64 * WAVES + tid; t < a.n; t += (int)gridDim.x * 64 * WAVES) {
-      const long x = a.lens[t] - a.len;
-      a.suffix[t] = x > 0 ? x : 0;
-    }
-  // Heads fastest, then row tiles: those of one head and range run together and on one XCD
-  // (with 8 heads), which reads the range's pages once.
-  const int h = (int)(blockIdx.x % (unsigned)L.H), tile = (int)(blockIdx.x / (unsigned)L.H), z = blockIdx.y;
-  const int n_rows = (int)a.n * a.gqa;  // below 2^25, checked on the host
-  const int k_begin = z * a.per, k_end = z == a.ranges - 1 ? a.len : min(a.len, k_begin + a.per);
-  const int n_steps = k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
-
-  // ---- this thread's item of a step, and its chain of loads ----------------
-  const int oct = tid % OCTS, quad = tid % 256 / OCTS;
-  const bool keys = BOTH || wave < 4, values = BOTH || wave >= 4;  // wave-uniform: what of the item this thread takes
-  const int ch = 8 * oct;
-  const int G = D / L.VG, vg = ch / L.VG;
-  // Nothing loaded is looked at before the step that needs it, and no load sits in a
-  // branch (addresses are clamped instead): the wave would wait for it there.
-  auto item_key = [&](int step) { return k_begin + step * KEYS + 4 * quad; };
-  auto item_off = [&](int step) { return item_key(step) & (L.BS - 1); };
-  auto load_blk = [&](int step) -> int {
-    const int kp = item_key(step);
+  __device__ __forceinline__ Items(const PrefixArgs& args, int head, int begin, int end, int id)
+      : a(args), h(head), k_begin(begin), k_end(end), oct(id % OCTS), quad(id / OCTS) {}
+  __device__ __forceinline__ int key(int step) const { return k_begin + step * KEYS + 4 * quad; }
+  __device__ __forceinline__ int off(int step) const { return key(step) & (a.L.BS - 1); }
+  __device__ __forceinline__ int load_blk(int step) const {
+    const int kp = key(step);
     return a.blocks[(kp < k_end - 1 ? kp : k_end - 1) >> a.bs_shift];
-  };
-  struct Head {
-    uint4 h;
-    int blk, rs;  // rs: the low word (slots are small, -1: none)
-  };
-  auto page_of = [&](int blk) { return (unsigned)blk < (unsigned long)L.nb ? (long)blk : 0l; };
-  auto load_head = [&](int blk) {
+  }
+  __device__ __forceinline__ long page_of(int blk) const { return (unsigned)blk < (unsigned long)a.L.nb ? (long)blk : 0l; }
+  __device__ __forceinline__ Head load_head(int blk) const {
     const long b = page_of(blk);
-    return Head{*(const uint4*)(a.pages + b * L.stride), blk, *(const int32_t*)(a.block_res + b)};
-  };
-  auto load_raw = [&](int step, const Head& x, Raw& w) {
+    return Head{*(const uint4*)(a.pages + b * a.L.stride), blk, *(const int32_t*)(a.block_res + b)};
+  }
+  // keys, values (wave-uniform): what of the item this thread takes; values alone use w.k.
+  __device__ __forceinline__ void load(int step, const Head& x, Raw& w, bool keys, bool values, bool both) const {
+    const Lay& L = a.L;
     const int rs = (unsigned)x.rs < (unsigned)a.res.rows ? x.rs : 0;
     w.rg = *(const int32_t*)(a.res_group + rs);  // the low word: groups are small
-    const int off = item_off(step), bits = tier_of(x.h.x & 0xffu);
+    const int ch = 8 * oct, G = D / L.VG, o = off(step), bits = tier_of(x.h.x & 0xffu);
     const int tpc_shift = a.bs_shift + 1 - (bits == 8 ? 3 : bits == 4 ? 2 : 1);
-    const int c = off >> tpc_shift;
+    const int c = o >> tpc_shift;
     long cb = page_of(x.blk) * L.stride + L.o_data;
-    bool ok = (unsigned)x.blk < (unsigned long)L.nb && item_key(step) < k_end;
+    bool ok = (unsigned)x.blk < (unsigned long)L.nb && key(step) < k_end;
     if (c > 0) {
       const Hdr hd{x.h.x & 0xffu, (int32_t)x.h.y, (int32_t)x.h.z, (int32_t)x.h.w};
       const uint32_t id = (uint32_t)hd.id(c - 1);
@@ -97,48 +81,50 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
     w.ok = ok;
     const int rowb = L.H * (D / 4) * bits;
     const uint8_t* pg = a.pages + page_of(x.blk) * L.stride;
-    // A quad that cannot be read takes its page's first bytes instead (dequantized to zero).
-    const uint8_t* kp = ok ? a.pages + cb + (long)(off & ((1 << tpc_shift) - 1)) * rowb + ((h * D + ch) * bits / 8 & ~7) : pg;
+    // An item that cannot be read takes its page's first bytes instead (dequantized to zero).
+    const uint8_t* kp = ok ? a.pages + cb + (long)(o & ((1 << tpc_shift) - 1)) * rowb + ((h * D + ch) * bits / 8 & ~7) : pg;
     const int step_b = ok ? rowb : 0;
     if (keys) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w.k[i] = *(const uint2*)(kp + i * step_b);
-      const int se = ((off >> a.kg_shift) * L.H + h) * D + ch;
+      const int se = ((o >> a.kg_shift) * L.H + h) * D + ch;
       w.ks = *(const uint4*)(pg + L.o_ks + 2 * se);
       w.km = *(const uint4*)(pg + L.o_km + 2 * se);
     }
     if (values) {
-      const int ve = (off * L.H + h) * G + vg;
+      const int ve = (o * L.H + h) * G + ch / L.VG;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        (BOTH ? w.v : w.k)[i] = *(const uint2*)(kp + i * step_b + step_b / 2);
+        (both ? w.v : w.k)[i] = *(const uint2*)(kp + i * step_b + step_b / 2);
         w.vs[i] = *(const uint16_t*)(pg + L.o_vs + 2 * (ve + i * L.H * G));
         w.vm[i] = *(const uint16_t*)(pg + L.o_vm + 2 * (ve + i * L.H * G));
       }
     }
-  };
-  // The item dequantized into LDS (keys past the range and blocks that cannot be read: zeros).
-  auto store_item = [&](int step, const Head& x, const Raw& w) {
-    uint8_t* const buf = lds + (BOTH ? 0 : (step & 1) * 3 * SIDE);
-    const int kp = item_key(step), off = item_off(step), bits = tier_of(x.h.x & 0xffu);
-    const int key0 = 4 * quad;
-    auto put_k = [&](int i, const float* x8) {
-      u4_t hi, lo;
+  }
+  __device__ __forceinline__ void put_k(uint8_t* buf, int i, const float* x8) const {
+    u4_t hi, lo;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const h2_t p = {(_Float16)x8[2 * e], (_Float16)x8[2 * e + 1]};
-        hi[e] = __builtin_bit_cast(uint32_t, p);
-        lo[e] = pack2<false>(x8[2 * e] - (float)p[0], x8[2 * e + 1] - (float)p[1]);
-      }
-      const int at = (key0 + i) * (2 * D) + 16 * (oct ^ k_swz<D>(key0 + i));
-      *(u4_t*)(buf + at) = hi;
-      *(u4_t*)(buf + SIDE + at) = lo;
-    };
-    auto put_v = [&](int i, const u4_t x) {
-      *(u4_t*)(buf + 2 * SIDE + (key0 + i) * (2 * D) + 16 * (oct ^ v_swz<D>(key0 + i))) = x;
-    };
+    for (int e = 0; e < 4; ++e) {
+      const h2_t p = {(_Float16)x8[2 * e], (_Float16)x8[2 * e + 1]};
+      hi[e] = __builtin_bit_cast(uint32_t, p);
+      lo[e] = pack2<false>(x8[2 * e] - (float)p[0], x8[2 * e + 1] - (float)p[1]);
+    }
+    const int k = 4 * quad + i, at = k * (2 * D) + 16 * (oct ^ k_swz<D>(k));
+    *(u4_t*)(buf + at) = hi;
+    *(u4_t*)(buf + SIDE + at) = lo;
+  }
+  __device__ __forceinline__ void put_v(uint8_t* buf, int i, const u4_t x) const {
+    const int k = 4 * quad + i;
+    *(u4_t*)(buf + 2 * SIDE + k * (2 * D) + 16 * (oct ^ v_swz<D>(k))) = x;
+  }
+  // The item dequantized into a step's K hi, K lo and V at `buf` (LDS or memory; keys past the
+  // range and blocks that cannot be read: zeros).
+  __device__ __forceinline__ void store(uint8_t* buf, int step, const Head& x, const Raw& w, bool keys, bool values,
+                                        bool both) const {
+    const Lay& L = a.L;
+    const int kp = key(step), o = off(step), bits = tier_of(x.h.x & 0xffu), ch = 8 * oct;
     const int sh = 8 * (((h * D + ch) * bits / 8) & 7);
-    auto rows = [&](auto width) {
+    auto rows = [&](auto width) __attribute__((always_inline)) {
       constexpr int B = decltype(width)::value;
       const uint32_t sw[4] = {w.ks.x, w.ks.y, w.ks.z, w.ks.w}, mw[4] = {w.km.x, w.km.y, w.km.z, w.km.w};
       if (keys) {
@@ -150,7 +136,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             x8[e] = __builtin_fmaf((float)c[e >> 1][e & 1], (float)u2h(sw[e >> 1])[e & 1], (float)u2h(mw[e >> 1])[e & 1]);
-          put_k(i, x8);
+          put_k(buf, i, x8);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -158,12 +144,12 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           h2_t c[4];
-          code_pairs<B>((BOTH ? w.v : w.k)[i], sh, c);
+          code_pairs<B>((both ? w.v : w.k)[i], sh, c);
           const h2_t vs = u2h(w.vs[i] * 0x10001u), vm = u2h(w.vm[i] * 0x10001u);
           u4_t v;
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[e], vs, vm));
-          put_v(i, v);
+          put_v(buf, i, v);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -176,222 +162,281 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
       const float z8[8] = {};
 #pragma unroll 1
       for (int i = n_live > 0 ? n_live : 0; i < 4; ++i) {
-        if (keys) put_k(i, z8);
-        if (values) put_v(i, u4_t{});
+        if (keys) put_k(buf, i, z8);
+        if (values) put_v(buf, i, u4_t{});
       }
     }
-    if (keys && w.ok && (unsigned)x.rs < (unsigned)a.res.rows && w.rg == off >> a.kg_shift) {  // rare: an open K group
+    if (keys && w.ok && (unsigned)x.rs < (unsigned)a.res.rows && w.rg == o >> a.kg_shift) {  // rare: an open K group
 #pragma unroll 1
       for (int i = 0; i < 4 && kp + i < k_end; ++i) {
         float x8[8];
-        ld_n<8>(a.res.ptr, a.res.dtype,
-                x.rs * a.res.s0 + (long)((off + i) & (L.KG - 1)) * a.res.s1 + h * a.res.s2 + ch, x8);
-        put_k(i, x8);
+        ld_n<8>(a.res.ptr, a.res.dtype, x.rs * a.res.s0 + (long)((o + i) & (L.KG - 1)) * a.res.s1 + h * a.res.s2 + ch, x8);
+        put_k(buf, i, x8);
       }
     }
-  };
+  }
+};
 
+// A lane's query row: row r of the (entry, GQA head) pairs of KV head h.
+struct Row {
+  int t, qh;
+  long q_row;
+  bool live;
+};
+__device__ __forceinline__ Row row_of(const PrefixArgs& a, int h, int r) {
+  const bool live = r < (int)a.n * a.gqa;  // below 2^25, checked on the host
+  const int t = live ? (int)((unsigned)r / (unsigned)a.gqa) : 0;
+  return Row{t, h * a.gqa + (live ? r - t * a.gqa : 0), a.q_rows ? a.q_rows[t] : t, live};
+}
+
+// The row's query as fragments: 16 bytes at a time, all requested together.
+template <int D, int NKB, bool QLO>
+__device__ __forceinline__ void load_query(Rows<D, false, NKB, 2, QLO>& w, const PrefixArgs& a, const Row& row, int hh) {
+  constexpr int NS = D / 16, QW = QLO ? 2 : 1;
+  w.set_scale(a.scale_log2);
+  const uint8_t* src = (const uint8_t*)a.q + (row.q_row * a.q_s0 + (long)row.qh * a.q_s1 + 8 * hh) * (2 * QW);
+  const uint32_t flip = a.scale_log2 < 0.f ? (QLO ? 0x80000000u : 0x80008000u) : 0u;
+  u4_t x[NS][QW];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < QW; ++i) x[s][i] = *(const u4_any_t*)(src + 32 * QW * s + 16 * i) ^ flip;
+  const bool bf = a.q_dtype == ECHOKV_BF16;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    if constexpr (QLO) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = __uint_as_float(x[s][e >> 2][e & 3]);
+        w.q[s][e] = (_Float16)y;
+        w.ql[s][e] = (_Float16)(y - (float)w.q[s][e]);
+      }
+    } else {
+      u4_t y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[e] = pack2<false>(__uint_as_float(x[s][0][e] << 16), __uint_as_float(x[s][0][e] & 0xffff0000u));
+      w.q[s] = __builtin_bit_cast(h8_t, bf ? y : x[s][0]);
+    }
+  }
+}
+
+// Scores of a step's keys from `left` on: -inf.
+template <int NKB>
+__device__ __forceinline__ void mask_tail(f16v_t* s, int left, int hh) {
+  left -= 4 * hh;
+  asm volatile("" : "+v"(left));  // keeps the compares in the caller's branch
+#pragma unroll
+  for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) < left ? s[kb][i] : -kInf;
+}
+
+// The wave's rows out: range z's partial ones, or normalized ones with their log-sum-exp.
+template <int D, int NKB, bool QLO>
+__device__ __forceinline__ void write_rows(Rows<D, false, NKB, 2, QLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
+  const float l = halves_sum(w.l);
+  asm volatile("" : "+v"(r));  // the row's place is found again, not kept through the loop
+  const Row row = row_of(a, h, r);
+  if (!row.live) return;
+  const bool direct = a.part != nullptr;
+  const long pr = ((long)z * a.n + row.t) * a.hq + row.qh;
+  if (hh == 0) {
+    if (direct) a.lse[row.q_row * a.hq + row.qh] = l == 0.f ? -kInf : w.m - w.kShift + __log2f(l);
+    else *(float2*)(a.ml + 2 * pr) = float2{w.m - w.kShift, l};
+  }
+  const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  float* dst = (direct ? a.part + row.q_row * a.p_s0 + (long)row.qh * a.p_s1 : a.acc + pr * D) + 4 * hh;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db) {
+    if (direct) w.acc[db] *= inv;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *(f4_any_t*)(dst + 32 * db + 8 * g) =
+          f4_t{w.acc[db][4 * g], w.acc[db][4 * g + 1], w.acc[db][4 * g + 2], w.acc[db][4 * g + 3]};
+  }
+}
+
+// Decode: the lengths behind the prefix, for the kernels that follow.
+__device__ __forceinline__ void write_suffix(const PrefixArgs& a) {
+  if (!a.suffix) return;
+  for (int t = (int)(blockIdx.x * blockDim.x + threadIdx.x); t < a.n; t += (int)(gridDim.x * blockDim.x)) {
+    const long x = a.lens[t] - a.len;
+    a.suffix[t] = x > 0 ? x : 0;
+  }
+}
+
+}  // namespace
+
+template <int D, bool QLO, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) void prefix_kernel(PrefixArgs a) {
+  static_assert(WAVES == 4 || WAVES == 8, "a thread takes its items' K and V, or one of them");
+  constexpr bool BOTH = WAVES == 4;
+  constexpr int KEYS = 8192 / D;           // keys per step: 256 items
+  constexpr int NKB = KEYS >= 64 ? 2 : 1;  // 32-key blocks per softmax update
+  using I = Items<D, KEYS>;
+  constexpr int SIDE = I::SIDE;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+
+  write_suffix(a);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int j = lane & 31, hh = lane >> 5;
+  // Heads fastest, then row tiles: those of one head and range run together and on one XCD
+  // (with 8 heads), which reads the range's pages once.
+  const int h = (int)(blockIdx.x % (unsigned)a.L.H), tile = (int)(blockIdx.x / (unsigned)a.L.H), z = blockIdx.y;
+  const int k_begin = z * a.per, k_end = z == a.ranges - 1 ? a.len : min(a.len, k_begin + a.per);
+  const int n_steps = k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
+  const bool keys = BOTH || wave < 4, values = BOTH || wave >= 4;  // wave-uniform
+  const I it(a, h, k_begin, k_end, (int)threadIdx.x % 256);
   Raw raw;
   Head head{}, head1{};
   int blk2 = 0;
   if (n_steps > 0) {
-    head = load_head(load_blk(0));
-    head1 = load_head(load_blk(1));
-    blk2 = load_blk(2);
-    load_raw(0, head, raw);
+    head = it.load_head(it.load_blk(0));
+    head1 = it.load_head(it.load_blk(1));
+    blk2 = it.load_blk(2);
+    it.load(0, head, raw, keys, values, BOTH);
   }
-
-  // ---- this lane's query row: 16 bytes at a time, all requested together ------
-  struct Row {
-    int t, qh;
-    long q_row;
-    bool live;
-  };
-  auto row_of = [&](int jj) {
-    const int r = tile * ROWS + 32 * wave + jj;
-    const bool live = r < n_rows;
-    const int t = live ? (int)((unsigned)r / (unsigned)a.gqa) : 0;
-    return Row{t, h * a.gqa + (live ? r - t * a.gqa : 0), a.q_rows ? a.q_rows[t] : t, live};
-  };
-  const bool active = tile * ROWS + 32 * wave < n_rows;
-  // As in prompt.hip: the scale positive.
-  constexpr float kTiny = 7.8886090522101181e-31f;
-  const float scale = fabsf(a.scale_log2) < kTiny ? kTiny : fabsf(a.scale_log2);
-  h8_t q[NS], ql[QLO ? NS : 1];
-  {
-    const Row row = row_of(j);
-    const uint8_t* src = (const uint8_t*)a.q + (row.q_row * a.q_s0 + (long)row.qh * a.q_s1 + 8 * hh) * (QLO ? 4 : 2);
-    const uint32_t flip = a.scale_log2 < 0.f ? (QLO ? 0x80000000u : 0x80008000u) : 0u;
-    u4_t w[NS][QLO ? 2 : 1];
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int i = 0; i < (QLO ? 2 : 1); ++i) w[s][i] = *(const u4_any_t*)(src + 32 * (QLO ? 2 : 1) * s + 16 * i) ^ flip;
-    const bool bf = a.q_dtype == ECHOKV_BF16;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      if constexpr (QLO) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = __uint_as_float(w[s][e >> 2][e & 3]);
-          q[s][e] = (_Float16)x;
-          ql[s][e] = (_Float16)(x - (float)q[s][e]);
-        }
-      } else {
-        u4_t y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = pack2<false>(__uint_as_float(w[s][0][e] << 16), __uint_as_float(w[s][0][e] & 0xffff0000u));
-        q[s] = __builtin_bit_cast(h8_t, bf ? y : w[s][0]);
-      }
-    }
-  }
-
-  f16v_t acc[NDB];
-#pragma unroll
-  for (int db = 0; db < NDB; ++db) acc[db] = f16v_t{};
-  float m_run = -kInf, lsum = 0.f;
+  const int r = (tile * WAVES + wave) * 32 + j;
+  const bool active = (tile * WAVES + wave) * 32 < (int)a.n * a.gqa;
+  Rows<D, false, NKB, 2, QLO> w;
+  load_query(w, a, row_of(a, h, r), hh);
+  w.clear();
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  // Slots are permuted by exclusive or, and LDS rows are whole multiples of their slots: a
-  // fragment's address is the first one's with the slot's bits flipped.
   const uint32_t k_lane = lds0 + k_at<D>(0, j, hh), v_lane = lds0 + 2 * SIDE + v_at<D>(0, lane);
 
-  // An item into LDS, then the words of the next one requested.
-  auto put_step = [&](int step) {
-    store_item(step, head, raw);
-    if (step + 1 < n_steps) {
-      head = head1;
-      load_raw(step + 1, head, raw);
-      head1 = load_head(blk2);
-      blk2 = load_blk(step + 3);
-    }
+  // The words of step `step` requested.
+  auto fetch = [&](int step) __attribute__((always_inline)) {
+    if (step >= n_steps) return;
+    head = head1;
+    it.load(step, head, raw, keys, values, BOTH);
+    head1 = it.load_head(blk2);
+    blk2 = it.load_blk(step + 2);
   };
-  if (!BOTH && n_steps > 0) put_step(0);
+  // Eight waves: two steps in LDS, the next one is written while this one is computed.
+  if (!BOTH && n_steps > 0) {
+    it.store(lds, 0, head, raw, keys, values, BOTH);
+    fetch(1);
+  }
   for (int step = 0; step < n_steps; ++step) {
     __syncthreads();  // every wave is done with the step before (eight waves: and this one is there)
-    if constexpr (BOTH) {
-      store_item(step, head, raw);
-      __syncthreads();
-      if (step + 1 < n_steps) {
-        head = head1;
-        load_raw(step + 1, head, raw);
-        head1 = load_head(blk2);
-        blk2 = load_blk(step + 3);
-      }
-    } else if (step + 1 < n_steps) {
-      put_step(step + 1);
+    const int put = BOTH ? step : step + 1;
+    const uint32_t buf = BOTH ? 0u : (uint32_t)((step & 1) * 3 * SIDE);
+    if (put < n_steps) {
+      it.store(lds + (BOTH ? 0 : (put & 1) * 3 * SIDE), put, head, raw, keys, values, BOTH);
+      if (BOTH) __syncthreads();
+      fetch(put + 1);
     }
     if (!active) continue;
-    const uint32_t buf = BOTH ? 0u : (uint32_t)((step & 1) * 3 * SIDE);
 #pragma unroll 1
     for (int sb = 0; sb < KEYS; sb += 32 * NKB) {
       const int left = k_end - (k_begin + step * KEYS + sb);  // keys of this block that there are
       if (left <= 0) break;
       f16v_t s[NKB];
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb) s[kb] = f16v_t{};
-      {
-        h8_t f[2][NKB];
-        auto load = [&](int u, h8_t* x) {  // channels 16 (u / 2) .. + 16 of K hi or lo
-#pragma unroll
-          for (int kb = 0; kb < NKB; ++kb)
-            x[kb] = k_read<D>((k_lane ^ 32 * (u >> 1)) + (u & 1) * SIDE + buf + sb * 2 * D, kb);
-        };
-        load(0, f[0]);
-#pragma unroll
-        for (int u = 0; u < 2 * NS; ++u) {
-          if (u + 1 < 2 * NS) load(u + 1, f[(u + 1) & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int kb = 0; kb < NKB; ++kb) s[kb] = mma<false>(f[u & 1][kb], q[u >> 1], s[kb]);
-          if constexpr (QLO) {
-            if (!(u & 1)) {
-#pragma unroll
-              for (int kb = 0; kb < NKB; ++kb) s[kb] = mma<false>(f[u & 1][kb], ql[u >> 1], s[kb]);
-            }
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      if (left < 32 * NKB) {
-        int mine = left - 4 * hh;
-        asm volatile("" : "+v"(mine));  // keeps the 32 compares in this branch
-#pragma unroll
-        for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) < mine ? s[kb][i] : -kInf;
-      }
-      float mx = -kInf;
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-      const float mt = halves_max(mx) * scale;
-      if (__builtin_amdgcn_ballot_w64(mt > m_run + 8.f)) {  // weights stay below 2^8 x 2^6
-        const float m_new = fmaxf(m_run, mt);
-        const float alpha = m_new == -kInf ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
-        lsum *= alpha;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) acc[db] *= alpha;
-        m_run = m_new;
-      }
-      const float ms = m_run == -kInf ? 0.f : m_run - kShift;
-      float sum[2] = {0.f, 0.f};
       u4_t p[2 * NKB];
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], scale, -ms));
-          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i + 1], scale, -ms));
-          sum[0] += x;
-          sum[1] += y;
-          p[2 * kb + (i >> 3)][(i & 7) >> 1] = pack2<false>(x, y);
-        }
-      lsum += sum[0] + sum[1];
-      {
-        constexpr int NG = NDB < 4 ? NDB : 4, NP = NDB / NG;
-        h8_t f[2][NG];
-        auto load = [&](int g, h8_t* x) {
-#pragma unroll
-          for (int i = 0; i < NG; ++i) x[i] = v_read<D>((v_lane ^ 64 * (g % NP * NG + i)) + buf + sb * 2 * D, g / NP);
-        };
-        load(0, f[0]);
-#pragma unroll
-        for (int g = 0; g < 2 * NKB * NP; ++g) {
-          if (g + 1 < 2 * NKB * NP) load(g + 1, f[(g + 1) & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            const int db = g % NP * NG + i;
-            acc[db] = mma<false>(f[g & 1][i], __builtin_bit_cast(h8_t, p[g / NP]), acc[db]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
+      w.template scores<SIDE>(k_lane + buf + sb * 2 * D, s);
+      if (left < 32 * NKB) mask_tail<NKB>(s, left, hh);
+      w.rescale(w.top(s));
+      w.template weights<false, SIDE>(s, p, 0, s);
+      w.template values<false>(p, v_lane + buf + sb * 2 * D, s);
     }
   }
+  write_rows(w, a, h, r, z, hh);
+}
 
-  const float l = halves_sum(lsum);
-  int jj = j;
-  asm volatile("" : "+v"(jj));  // the row's place is found again, not kept through the loop
-  const auto [t, qh, q_row, live] = row_of(jj);
-  if (!live) return;
-  const bool direct = a.part != nullptr;
-  const long pr = ((long)z * a.n + t) * a.hq + qh;
-  if (hh == 0) {
-    if (direct) a.lse[q_row * a.hq + qh] = l == 0.f ? -kInf : m_run - kShift + __log2f(l);
-    else *(float2*)(a.ml + 2 * pr) = float2{m_run - kShift, l};
-  }
-  const float inv = !direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
-  float* dst = (direct ? a.part + q_row * a.p_s0 + (long)qh * a.p_s1 : a.acc + pr * D) + 4 * hh;
+// One workgroup per (64-key tile, KV head): its K hi, K lo and V into the workspace.
+template <int D>
+__global__ __launch_bounds__(256) void prefix_pack_kernel(PrefixArgs a) {
+  using I = Items<D, kPackKeys>;
+  write_suffix(a);
+  const int h = (int)(blockIdx.x % (unsigned)a.L.H), tile = (int)(blockIdx.x / (unsigned)a.L.H);
+  const I it(a, h, tile * kPackKeys, min(a.len, (tile + 1) * kPackKeys), (int)threadIdx.x);
+  if (4 * it.quad >= kPackKeys) return;  // head size 64: half of the threads
+  Raw raw;
+  const Head head = it.load_head(it.load_blk(0));
+  it.load(0, head, raw, true, true, true);
+  it.store(a.pack + ((long)tile * a.L.H + h) * (3 * I::SIDE), 0, head, raw, true, true, true);
+}
+
+template <int D>
+__global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
+  constexpr int WAVES = 8, KEYS = kPackKeys, NKB = 2, SIDE = KEYS * D * 2;
+  constexpr int KDMA = 2 * SIDE / 1024 / WAVES, VDMA = SIDE / 1024 / WAVES;
+  // LDS: the keys (hi, lo) of two steps, then the values of two.
+  constexpr int V0 = 4 * SIDE;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int j = lane & 31, hh = lane >> 5;
+  const int h = (int)(blockIdx.x % (unsigned)a.L.H), tile = (int)(blockIdx.x / (unsigned)a.L.H), z = blockIdx.y;
+  const int k_begin = z * a.per, k_end = z == a.ranges - 1 ? a.len : min(a.len, k_begin + a.per);
+  const int n_steps = k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+  const uint8_t* tiles = a.pack + ((long)(k_begin / KEYS) * a.L.H + h) * (3 * SIDE);
+  auto issue = [&](int step, bool val) __attribute__((always_inline)) {
+    const int n = val ? VDMA : KDMA;
+    const uint8_t* from = uniform_ptr(tiles + (long)step * a.L.H * (3 * SIDE) + (val ? 2 * SIDE : 0) + 1024 * n * wave);
+    const uint32_t to = lds0 + (uint32_t)((val ? V0 + (step & 1) * SIDE : (step & 1) * 2 * SIDE) + 1024 * n * wave);
 #pragma unroll
-  for (int db = 0; db < NDB; ++db) {
-    if (direct) acc[db] *= inv;
-#pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *(f4_any_t*)(dst + 32 * db + 8 * g) = f4_t{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+    for (int i = 0; i < n; ++i) dma16(from, 1024 * i + 16 * lane, to + 1024 * i);
+  };
+  if (n_steps > 0) {
+    issue(0, false);
+    issue(0, true);
+    if (n_steps > 1) issue(1, false);
   }
+  const int r = (tile * WAVES + wave) * 32 + j;
+  const bool active = (tile * WAVES + wave) * 32 < (int)a.n * a.gqa;
+  Rows<D, false, NKB, 2, false> w;
+  load_query(w, a, row_of(a, h, r), hh);
+  w.clear();
+  const uint32_t k_lane = lds0 + k_at<D>(0, j, hh), v_lane = lds0 + V0 + v_at<D>(0, lane);
+
+  // As in prompt.hip: at `step` the keys of `step` + 1 and the values of `step` have landed.
+  auto advance = [&](int step) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (step + 2 < n_steps) issue(step + 2, false);
+    if (step + 1 < n_steps) issue(step + 1, true);
+  };
+  f16v_t s0[NKB], s1[NKB];
+  float mt = -kInf;
+  const int tail = (k_end - k_begin) % KEYS;
+  auto body = [&](int step, f16v_t* cur, f16v_t* nxt) __attribute__((always_inline)) {
+    advance(step);
+    w.rescale(mt);
+    u4_t p[2 * NKB];
+    w.template weights<true, SIDE>(cur, p, k_lane + (uint32_t)(((step + 1) & 1) * 2 * SIDE), nxt);
+    mt = w.template values<true>(p, v_lane + (uint32_t)((step & 1) * SIDE), nxt);
+    if (tail && step + 2 == n_steps) {
+      mask_tail<NKB>(nxt, tail, hh);
+      mt = w.top(nxt);
+    }
+  };
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (active && n_steps > 0) {
+    w.template scores<SIDE>(k_lane, s0);
+    if (tail && n_steps == 1) mask_tail<NKB>(s0, tail, hh);
+    mt = w.top(s0);
+    int step = 0;
+    for (; step + 2 < n_steps; step += 2) {
+      body(step, s0, s1);
+      body(step + 1, s1, s0);
+    }
+    if (step + 1 < n_steps) {
+      body(step++, s0, s1);
+      s0[0] = s1[0];
+      s0[1] = s1[1];
+    }
+    advance(step);
+    w.rescale(mt);
+    u4_t p[2 * NKB];
+    w.template weights<false, SIDE>(s0, p, 0, s0);
+    w.template values<false>(p, v_lane + (uint32_t)((step & 1) * SIDE), s0);
+  } else {
+    for (int step = 0; step < n_steps; ++step) advance(step);
+  }
+  write_rows(w, a, h, r, z, hh);
 }
 
 template <int D, bool QLO, int WAVES>
@@ -407,12 +452,27 @@ static hipError_t launch_t(const PrefixArgs& a, hipStream_t s) {
 }
 
 template <int D>
+static hipError_t launch_packed(const PrefixArgs& a, hipStream_t s) {
+  constexpr int lds = 6 * kPackKeys * D * 2;
+  static std::atomic<uint64_t> attr_done{0};
+  hipError_t e = ensure_lds_limit((const void*)prefix_flash_kernel<D>, lds, &attr_done);
+  if (e != hipSuccess) return e;
+  const unsigned packs = (unsigned)((a.len + kPackKeys - 1) / kPackKeys * a.L.H);
+  hipLaunchKernelGGL(prefix_pack_kernel<D>, dim3(packs), dim3(256), 0, s, a);
+  if ((e = hipGetLastError()) != hipSuccess) return e;
+  const dim3 grid((unsigned)((a.n * a.gqa + 255) / 256 * a.L.H), (unsigned)a.ranges);
+  hipLaunchKernelGGL(prefix_flash_kernel<D>, grid, dim3(512), lds, s, a);
+  return hipGetLastError();
+}
+
+template <int D>
 static hipError_t launch_d(const PrefixArgs& a, hipStream_t s) {
   if (a.q_dtype == ECHOKV_F32) {
     if constexpr (D == 256) return hipErrorInvalidValue;  // its registers do not fit: attend_any.hip
     else return launch_t<D, true, 4>(a, s);
   }
   if constexpr (D == 256) return launch_t<D, false, 4>(a, s);
+  else if (a.pack) return launch_packed<D>(a, s);
   else return prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa) == 256 ? launch_t<D, false, 8>(a, s) : launch_t<D, false, 4>(a, s);
 }
 

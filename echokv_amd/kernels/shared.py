@@ -95,6 +95,17 @@ def shared_workspace_bytes(store, num_q_heads: int, num_seqs: int, prefix_len: i
                      num_splits)
 
 
+def suffix_blocks(store, num_seqs: int) -> int:
+    """Blocks per split of the tokens behind the prefix when the caller names none: 128 tokens
+    for few sequences (up to 64 groups of four KV heads), else 256. A split is a serial chain of
+    tiles, and these results depend on the batch anyway. us a call at 128 / 256 / 1024 tokens:
+    4 sequences of 500-2000 behind 2048 tokens 32 / 40 / 84, 16 of them 40 / 45 / 90, 64
+    73 / 68 / 115, 128 of 100-2000 104 / 100 / 141."""
+    L = store.layout
+    tokens = 128 if num_seqs * -(-L.num_kv_heads // 4) <= 64 else 256
+    return max(1, tokens // L.block_size)
+
+
 def suffix_splits(max_blocks: int, block_size: int, prefix_len: int, blocks_per_split: int,
                   max_len: int | None) -> int:
     """Splits of the tokens behind the prefix for sequences of at most ``max_blocks`` blocks (and
@@ -105,7 +116,7 @@ def suffix_splits(max_blocks: int, block_size: int, prefix_len: int, blocks_per_
 
 
 def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                         prefix_len: int, softmax_scale: float, blocks_per_split: int = dec.BLOCKS_PER_SPLIT,
+                         prefix_len: int, softmax_scale: float, blocks_per_split: int | None = None,
                          q_rows: torch.Tensor | None = None, bt_rows: torch.Tensor | None = None,
                          blocks: torch.Tensor | None = None, out: torch.Tensor | None = None,
                          max_len: int | None = None, num_splits: int | None = None,
@@ -117,13 +128,14 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
     Arguments as ``decode_attention``'s; ``seq_lens[i]`` counts the prefix, and row
     ``bt_rows[i]`` of the block table begins with the shared blocks. ``blocks``: their list (int32), by
     default the first row of the table. A sequence shorter than ``prefix_len`` (length 0:
-    graph padding) leaves its row untouched. ``num_splits`` and ``max_len``'s default splits cut the
-    tokens behind the prefix. ``workspace``: uint8, ``shared_workspace_bytes(...)``; by default the
+    graph padding) leaves its row untouched. ``num_splits`` and ``blocks_per_split`` (default
+    ``suffix_blocks``) cut the tokens behind the prefix. ``workspace``: uint8, ``shared_workspace_bytes(...)``; by default the
     call allocates it. A prefix of 0 tokens is plain decode."""
     prefix_len = int(prefix_len)
     if prefix_len == 0:
-        return dec.decode_attention(store, query, block_table, seq_lens, softmax_scale, blocks_per_split, q_rows,
-                                    bt_rows, out, max_len, num_splits, None, tier, True, tier_mask)
+        return dec.decode_attention(store, query, block_table, seq_lens, softmax_scale,
+                                    blocks_per_split or dec.BLOCKS_PER_SPLIT, q_rows, bt_rows, out, max_len, num_splits,
+                                    None, tier, True, tier_mask)
     L = store.layout
     if prefix_len < 0 or prefix_len % L.block_size:
         raise ValueError(f"prefix_len must be a multiple of the block size {L.block_size}, got {prefix_len}")
@@ -139,6 +151,8 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
         block_table = block_table.to(torch.int32).contiguous()
     if s and blocks is None and block_table.shape[0] == 0:
         raise ValueError("the block table has no row to take the shared blocks from")
+    if blocks_per_split is None:
+        blocks_per_split = suffix_blocks(store, s)
     if num_splits is None:
         num_splits = suffix_splits(block_table.shape[1], L.block_size, prefix_len, blocks_per_split, max_len)
     need = shared_workspace_bytes(store, hq, s, prefix_len, int(num_splits))

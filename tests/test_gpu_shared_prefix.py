@@ -124,6 +124,19 @@ def test_prefix_rows_and_ranges(device, rows, gqa, n):
     check_prefix(c, q, part, lse, n, c.d ** -0.5)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(d=64), dict(bs=64, kg=32, vg=64), dict(d=256)], ids=str)
+@pytest.mark.parametrize("rows,n", [(4200, 200), (4200, 63), (300, 64), (300, 65), (300, 128), (300, 2100), (700, 1)])
+def test_prefix_of_many_rows(device, kw, rows, n):
+    """Rows enough that the prefix is dequantized into the workspace first, one range and several."""
+    print(f"[prefix] many rows {kw} {rows} {n}", flush=True)
+    c = Cache(device, n, [], tiers=(4,) if n > 500 else (4, 8, 2), outliers=True, seed=rows + n, **kw)
+    for dtype in (BF16, F16):
+        q = c.queries(rows, 4, dtype)
+        part, lse = prefix_attention(c.store, q, c.blocks, n, c.d ** -0.5)
+        torch.cuda.synchronize()
+        check_prefix(c, q, part, lse, n, c.d ** -0.5)
+
+
 @pytest.mark.parametrize("scale", [-0.088, 0.0, 0.9])
 def test_prefix_scales(device, scale):
     c = Cache(device, 300, [], bs=64, kg=32)
@@ -160,7 +173,7 @@ def test_decode_matches_float64(device, kw, tiers):
         check_decode(c, q, out, c.lens, c.d ** -0.5)
 
 
-@pytest.mark.parametrize("seqs", [1, 2, 17, 64, 130])
+@pytest.mark.parametrize("seqs", [1, 2, 17, 64, 130, 260])
 @pytest.mark.parametrize("prefix", [64, 1024, 8192])
 def test_decode_batches(device, seqs, prefix):
     print(f"[shared] {seqs} behind {prefix}", flush=True)

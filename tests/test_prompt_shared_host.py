@@ -149,6 +149,7 @@ def test_shared_python_refusals(lib):
     assert sh._blocks(store, table[0], 49).numel() == 4
     with pytest.raises(ValueError):
         sh._workspace(torch.zeros(10, dtype=torch.uint8), 11, CPU)
+    assert [sh.suffix_blocks(store, n) for n in (1, 64, 65)] == [8, 8, 16]
     assert sh.suffix_splits(8, 16, 64, 16, None) == 4
     assert sh.suffix_splits(4096, 16, 64, 16, None) == 64
 
