@@ -242,7 +242,8 @@ __global__ __launch_bounds__(256) void prefix_any_kernel(PrefixArgs a) {
   const bool live = r < a.n * a.gqa;
   const long t = live ? r / a.gqa : 0;
   const int qh = h * a.gqa + (live ? (int)(r % a.gqa) : 0);
-  const long q_row = a.q_rows ? a.q_rows[t] : t;
+  // A sequence shorter than the prefix (graph padding): its row index may be any.
+  const long q_row = a.lens && a.lens[t] < a.len ? 0 : a.q_rows ? a.q_rows[t] : t;
   const int k_begin = z * a.per, k_end = z == a.ranges - 1 ? a.len : min(a.len, k_begin + a.per);
   f4_t q[S::NJ];
   load_q<DP>(a.q, a.q_dtype, q_row * a.q_s0 + (long)qh * a.q_s1, L.D, a.scale_log2, c, q);

@@ -177,7 +177,9 @@ struct Items {
   }
 };
 
-// A lane's query row: row r of the (entry, GQA head) pairs of KV head h.
+// A lane's query row: row r of the (entry, GQA head) pairs of KV head h. A sequence shorter than
+// the prefix (graph padding) is not asked for its row index, which may be any: it computes with
+// query row 0 into its workspace rows, and the join leaves them.
 struct Row {
   int t, qh;
   long q_row;
@@ -186,7 +188,8 @@ struct Row {
 __device__ __forceinline__ Row row_of(const PrefixArgs& a, int h, int r) {
   const bool live = r < (int)a.n * a.gqa;  // below 2^25, checked on the host
   const int t = live ? (int)((unsigned)r / (unsigned)a.gqa) : 0;
-  return Row{t, h * a.gqa + (live ? r - t * a.gqa : 0), a.q_rows ? a.q_rows[t] : t, live};
+  const long len = a.lens ? a.lens[t] : a.len, q_row = a.q_rows ? a.q_rows[t] : t;
+  return Row{t, h * a.gqa + (live ? r - t * a.gqa : 0), len < a.len ? 0 : q_row, live};
 }
 
 // The row's query as fragments: 16 bytes at a time, all requested together.

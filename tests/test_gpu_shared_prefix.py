@@ -211,6 +211,27 @@ def test_decode_rows_of_other_sequences_stay(device):
         assert (out[row] == 9.0).all()
 
 
+@pytest.mark.parametrize("d,seqs,prefix", [(128, 6, 64), (96, 6, 64), (128, 200, 4096)])
+def test_padding_may_name_any_row(device, d, seqs, prefix):
+    """Entries of length 0 or shorter than the prefix: their row indices are not followed."""
+    print(f"[shared] padding {d} {seqs}", flush=True)
+    c = Cache(device, prefix, [30, 5], d=d, vg=32 if d == 128 else 24)
+    q = c.queries(2, 4, F16)
+    q_rows, bt_rows, lens = [0, 1], [1, 0], [prefix + 5, prefix + 30]
+    for i in range(seqs - 2):
+        q_rows.append((-1, 1 << 40, -(1 << 40))[i % 3])
+        bt_rows.append((1 << 40, -1, 7)[i % 3])
+        lens.append((0, prefix - 1)[i % 2])
+    out = torch.zeros_like(q)
+    shared_prefix_decode(c.store, q, c.table, torch.tensor(lens, device=device), prefix, c.d ** -0.5, out=out,
+                         q_rows=torch.tensor(q_rows, device=device), bt_rows=torch.tensor(bt_rows, device=device),
+                         blocks=c.blocks)
+    torch.cuda.synchronize()
+    for row in range(2):
+        k, v = c.tokens(bt_rows[row], lens[row])
+        check(out[row : row + 1], Rows(q[row : row + 1], k, v, [lens[row]], c.d ** -0.5), **BOUND)
+
+
 def test_no_prefix_is_plain_decode(device):
     c = Cache(device, 0, [30, 5], bs=16)
     q = c.queries(2, 4, F16)
