@@ -686,8 +686,10 @@ bool prefix_packed(const echokv_layout* L, int hq, int q_dtype, int64_t n, int64
 
 bool prefix_shape_ok(const echokv_layout* L, int hq, int64_t n, int64_t len) {
   if (!lay_ok(L) || L->head_size > ek::kMaxAnyD || hq <= 0 || hq % L->num_kv_heads) return false;
-  // Grids: (rows / 64) x heads x ranges workgroups, rows / 4 waves of the join.
-  return n >= 0 && n <= INT32_MAX / 64 / hq && len >= 0 && len <= INT32_MAX - 1024;
+  // Grids: (rows / 64) x heads x ranges workgroups, rows / 4 waves of the join. The kernels' key
+  // positions are 32 bits: a range's end is up to 128 keys a range past the last key, a step and
+  // its two successors further.
+  return n >= 0 && n <= INT32_MAX / 64 / hq && len >= 0 && len <= INT32_MAX - 16384;
 }
 
 // Float32 rows of `hq` heads and their (max, sum) pairs, behind one another.

@@ -142,6 +142,12 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
     query = _query(store, query)
     hq, d = query.shape[1:]
     s = seq_lens.shape[0]
+    if q_rows is not None and q_rows.shape[0] < s or bt_rows is not None and bt_rows.shape[0] < s:
+        raise ValueError(f"{s} sequences, fewer row indices")
+    if bt_rows is None and block_table.shape[0] < s:
+        raise ValueError(f"{s} sequences, {block_table.shape[0]} block-table rows")
+    if out is not None and out.shape[0] < (s if q_rows is None else 1):
+        raise ValueError(f"{s} sequences, {out.shape[0]} output rows")
     _lib.require_current(query, block_table, seq_lens, q_rows, bt_rows, blocks, out, workspace, store.pages)
     if q_rows is None and query.shape[0] < s:
         raise ValueError(f"{s} sequences, {query.shape[0]} query rows")

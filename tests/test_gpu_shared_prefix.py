@@ -232,6 +232,26 @@ def test_padding_may_name_any_row(device, d, seqs, prefix):
         check(out[row : row + 1], Rows(q[row : row + 1], k, v, [lens[row]], c.d ** -0.5), **BOUND)
 
 
+@pytest.mark.parametrize("d,dtype", [(128, F16), (128, BF16), (128, F32), (96, F16)], ids=str)
+@pytest.mark.parametrize("prefix,rows", [(64, 3), (4096, 3), (4096, 200)])
+def test_nan_queries_and_scales(device, d, dtype, prefix, rows):
+    """A NaN in a query row, or as the softmax scale, makes its rows NaN and no others."""
+    print(f"[shared] nan {d} {prefix} {rows}", flush=True)
+    c = Cache(device, prefix, [0] * rows, d=d, vg=32 if d == 128 else 24)
+    q = c.queries(rows, 4, dtype)
+    q[1, 2, 5] = float("nan")
+    bad = torch.zeros(rows, q.shape[1], dtype=torch.bool, device=device)
+    bad[1, 2] = True
+    lens = torch.tensor(c.lens, device=device)
+    for scale, want in ((c.d ** -0.5, bad), (float("nan"), torch.ones_like(bad))):
+        part, lse = prefix_attention(c.store, q, c.blocks, prefix, scale)
+        out = shared_prefix_decode(c.store, q, c.table, lens, prefix, scale)
+        torch.cuda.synchronize()
+        assert torch.equal(lse.isnan(), want)
+        for rows_out in (part, out):
+            assert torch.equal(rows_out.isnan().all(-1), want) and torch.equal(rows_out.isnan().any(-1), want)
+
+
 def test_no_prefix_is_plain_decode(device):
     c = Cache(device, 0, [30, 5], bs=16)
     q = c.queries(2, 4, F16)

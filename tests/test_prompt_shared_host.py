@@ -118,6 +118,7 @@ def _shared(lib, entry, L=None, **kw):
 
 def test_prefix_entry_rejects_bad_arguments(lib):
     for kw, code in ((dict(hq=30), 2), (dict(n=-1), 2), (dict(prefix=-1), 2), (dict(prefix=1 << 40), 2), (dict(n=1 << 40), 2),
+                     (dict(prefix=(1 << 31) - 16384), 2),
                      (dict(dtype=5), 3), (dict(blocks=None), 1), (dict(out=None), 1), (dict(lse=None), 1),
                      (dict(prefix=4096, bytes=1000), 1), (dict(prefix=4096, ws=None), 1),
                      (dict(prefix=4096, ws=C.c_void_p(8)), 1), (dict(n=0), 0)):
@@ -142,6 +143,13 @@ def test_shared_python_refusals(lib):
     for bad in ((q, table, lens, 60), (q, table, lens, -16), (q[..., :64], table, lens, 64), (q[:, :3], table, lens, 64)):
         with pytest.raises(ValueError):
             sh.shared_prefix_decode(store, *bad, 0.1)
+    two = torch.zeros(2, dtype=torch.int64)
+    for kw in (dict(q_rows=two), dict(bt_rows=two), dict(out=torch.zeros(2, 8, 128)),
+               dict(out=torch.zeros(0, 8, 128), q_rows=torch.zeros(3))):
+        with pytest.raises(ValueError):
+            sh.shared_prefix_decode(store, q, table, lens, 64, 0.1, **kw)
+    with pytest.raises(ValueError, match="block-table"):
+        sh.shared_prefix_decode(store, q, table[:2], lens, 64, 0.1)
     with pytest.raises(ValueError):
         sh.prefix_attention(store, q, table[0], -1, 0.1)
     with pytest.raises(ValueError):
