@@ -22,14 +22,14 @@ class Cache:
     sequence's own ``tails`` tokens behind it."""
 
     def __init__(self, device, prefix, tails, h=2, d=128, bs=16, kg=16, vg=32, mem_bits=8, tiers=(4,), dtype=F16,
-                 seed=0, outliers=False):
+                 seed=0, outliers=False, spare=0):
         g = torch.Generator(device=device)
         g.manual_seed(seed)
         rng = np.random.default_rng(seed)
         self.prefix, self.tails, self.h, self.d, self.bs, self.device = prefix, tails, h, d, bs, device
         shared = -(-prefix // bs)
         own = [-(-n // bs) for n in tails]
-        nb = shared + sum(own) + 3
+        nb = shared + sum(own) + 3 + spare
         perm = rng.permutation(nb)
         self.table_np = np.full((max(1, len(tails)), shared + max(own, default=0) + 1), perm[-1], np.int64)
         self.table_np[:, :shared] = perm[:shared]
@@ -250,6 +250,24 @@ def test_nan_queries_and_scales(device, d, dtype, prefix, rows):
         assert torch.equal(lse.isnan(), want)
         for rows_out in (part, out):
             assert torch.equal(rows_out.isnan().all(-1), want) and torch.equal(rows_out.isnan().any(-1), want)
+
+
+@pytest.mark.parametrize("d,seqs,prefix", [(128, 3, 512), (96, 3, 512), (128, 200, 4096)])
+def test_pages_past_32_bits(device, d, seqs, prefix):
+    """Blocks all over a cache of more than 2^32 bytes."""
+    print(f"[shared] far pages {d} {seqs}", flush=True)
+    h, vg = 8, 32 if d == 128 else 24
+    spare = (6 << 30) // (16 * TieredLayout.per_token_bytes(h, d, 8, 16, vg))
+    c = Cache(device, prefix, [5] * seqs, h=h, d=d, vg=vg, spare=spare)
+    assert int(c.table_np.max()) * c.store.layout.page_bytes > 1 << 32
+    q = c.queries(seqs, 4, F16)
+    part, lse = prefix_attention(c.store, q, c.blocks, prefix, c.d ** -0.5)
+    out = shared_prefix_decode(c.store, q, c.table, torch.tensor(c.lens, device=device), prefix, c.d ** -0.5)
+    torch.cuda.synchronize()
+    check_prefix(c, q[:3], part[:3], lse[:3], prefix, c.d ** -0.5)
+    for i in (0, seqs - 1):
+        k, v = c.tokens(i, c.lens[i])
+        check(out[i : i + 1], Rows(q[i : i + 1], k, v, [c.lens[i]], c.d ** -0.5), **BOUND)
 
 
 def test_no_prefix_is_plain_decode(device):
