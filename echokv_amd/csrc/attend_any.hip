@@ -10,8 +10,6 @@
 // operands are: lane group c takes channels 16 j + 4 c .. + 4 of the score products (one
 // 16-byte read each), and keys 4 c + i of the value products, which is where the S^T
 // accumulator holds them, so P^T needs no exchange.
-//
-// Bound by the float32 matrix rate (1/16 of the 16-bit one) on long prompts.
 #include "items.h"
 
 namespace ek {
@@ -141,21 +139,39 @@ __device__ __forceinline__ void load_q(const void* q, int dtype, long at, int D,
 
 }  // namespace
 
-// One workgroup per (tile, 64 of its rows, KV head); heads fastest.
-template <int DP>
+// One workgroup per (tile, 64 / GROUPS of its rows, KV head); heads fastest, then tiles (longest
+// first) or, with two groups, the tile's parts. GROUPS 2: waves 2 and 3 take the same rows as 0 and
+// 1, over the odd steps of keys.
+//
+// A step is a chain (its rows stored, two barriers, products that wait for one another) of about
+// 3 us whatever runs beside it, so with few workgroups a wave's number of steps is the time: two
+// groups halve it, and stage each key for 32 rows instead of 64. They are taken up to three
+// workgroups (of 64 rows) a CU, one above head size 128, whose registers leave room for one. us
+// with one group / with two, 8 KV heads of GQA 4, float32: D 96, 300 tokens (160 workgroups)
+// 36 / 26, 100 + 400 + 700 tokens (624) 97 / 76, 2000 (1008) 316 / 366, 4000 (2000) 1165 / 1338;
+// D 128, 300 (160) 43 / 31, 1000 (512) 186 / 132, 2000 (1008) 390 / 462; D 64 (4 of GQA 8), 1500
+// (752) 157 / 139, 3000 (1504) 425 / 467; D 256 (2 of GQA 4), 1000 (128) 271 / 171, 2000 (252)
+// 532 / 350, 4000 (500) 1110 / 1309.
+// Bound by the chain, then by the float32 matrix rate: 4000 tokens at D 96 run at 84 TFLOP/s of
+// causal products, a library product of 4096^3 at 132.
+template <int DP, int GROUPS>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_any_kernel(PromptArgs a) {
   using S = Steps<DP>;
-  __shared__ __attribute__((aligned(16))) float kt[S::KEYS * S::PITCH], vt[S::KEYS * S::PITCH];
+  constexpr int ROWS = kRows / GROUPS, KEYS = GROUPS * S::KEYS;
+  __shared__ __attribute__((aligned(16))) float kv[2 * KEYS * S::PITCH];
+  float *const kt = kv, *const vt = kv + KEYS * S::PITCH;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, c = lane >> 4;
   const int h = (int)(blockIdx.x % a.H);
-  const int32_t* td = a.tiles + 4 * (long)(blockIdx.x / a.H);
+  const int parts = (a.tile_m * a.gqa + ROWS - 1) / ROWS, at_tile = (int)(blockIdx.x / a.H);
+  const int tile = GROUPS == 1 ? at_tile % a.n_tiles : at_tile / parts;
+  const int32_t* td = a.tiles + 4 * (long)tile;
   const long row0 = td[0];
   const int seq = td[1], t0 = td[2], n_rows = td[3] * a.gqa;
-  const int first = (int)blockIdx.y * kRows;
+  const int first = (GROUPS == 1 ? at_tile / a.n_tiles : at_tile % parts) * ROWS;
   if (first >= n_rows) return;
-  const int last = min(first + kRows, n_rows) - 1;
+  const int last = min(first + ROWS, n_rows) - 1;
   const int kv_end = min(seq, t0 + last / a.gqa + 1);  // keys that any row sees
-  const int r = first + 16 * (tid >> 6) + n;
+  const int r = first + (16 * (tid >> 6) & (ROWS - 1)) + n, group = tid >> 6 >= ROWS / 16;
   const bool live = r < n_rows;
   const int tok = t0 + (live ? r / a.gqa : 0), qh = h * a.gqa + (live ? r % a.gqa : 0);
   const int lim = live ? tok + 1 : 0;
@@ -164,7 +180,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_any_kernel(Promp
   State<DP> st;
   st.init();
   // A step's rows are requested while the one before is computed.
-  constexpr int ITEMS = S::KEYS * (DP / 4), NI = (ITEMS + 255) / 256;
+  constexpr int ITEMS = KEYS * (DP / 4), NI = (ITEMS + 255) / 256;
   float x[NI][4], y[NI][4];
   auto fetch = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
@@ -177,7 +193,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_any_kernel(Promp
     }
   };
   fetch(0);
-  for (int kb = 0; kb < kv_end; kb += S::KEYS) {
+  for (int kb = 0; kb < kv_end; kb += KEYS) {
     __syncthreads();
     bool odd = false;
 #pragma unroll
@@ -190,8 +206,30 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void prompt_any_kernel(Promp
       *(f4_t*)&vt[key * S::PITCH + ch] = there ? f4_t{y[u][0], y[u][1], y[u][2], y[u][3]} : f4_t{0.f, 0.f, 0.f, 0.f};
     }
     const int any_odd = __syncthreads_or(odd);
-    if (kb + S::KEYS < kv_end) fetch(kb + S::KEYS);
-    step_any<DP>(st, q, kt, vt, kb, lim, any_odd != 0, lane);
+    if (kb + KEYS < kv_end) fetch(kb + KEYS);
+    const int at = group * S::KEYS;
+    if (GROUPS == 1 || kb + at < kv_end)
+      step_any<DP>(st, q, kt + at * S::PITCH, vt + at * S::PITCH, kb + at, lim, any_odd != 0, lane);
+  }
+  if constexpr (GROUPS == 2) {  // the groups' rows added
+    constexpr int N = 4 * S::NJ;
+    float* const x = kv + (tid >> 6 & 1) * 64 * (N + 2) + lane;
+    __syncthreads();
+    if (group) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[64 * e] = st.acc[e >> 2][e & 3];
+      x[64 * N] = st.m;
+      x[64 * (N + 1)] = st.l;
+    }
+    __syncthreads();
+    if (group) return;
+    const float m1 = x[64 * N], top = fmaxf(st.m, m1);
+    const float w0 = top == -kInf ? 1.f : __builtin_amdgcn_exp2f(st.m - top);
+    const float w1 = top == -kInf ? 1.f : __builtin_amdgcn_exp2f(m1 - top);
+#pragma unroll
+    for (int e = 0; e < N; ++e) st.acc[e >> 2][e & 3] = st.acc[e >> 2][e & 3] * w0 + x[64 * e] * w1;
+    st.m = top;
+    st.l = st.l * w0 + x[64 * (N + 1)] * w1;
   }
   float l = st.l + __shfl_xor(st.l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -389,13 +427,20 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
   }
 }
 
-hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((long)a.n_tiles * a.H), (unsigned)(((long)a.tile_m * a.gqa + kRows - 1) / kRows));
-  if (a.D <= 64) hipLaunchKernelGGL(prompt_any_kernel<64>, grid, dim3(256), 0, s, a);
-  else if (a.D <= 96) hipLaunchKernelGGL(prompt_any_kernel<96>, grid, dim3(256), 0, s, a);
-  else if (a.D <= 128) hipLaunchKernelGGL(prompt_any_kernel<128>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(prompt_any_kernel<256>, grid, dim3(256), 0, s, a);
+template <int GROUPS>
+static hipError_t launch_prompt_any_t(const PromptArgs& a, hipStream_t s) {
+  constexpr int rows = kRows / GROUPS;
+  const dim3 grid((unsigned)((long)a.n_tiles * a.H * (((long)a.tile_m * a.gqa + rows - 1) / rows)));
+  if (a.D <= 64) hipLaunchKernelGGL((prompt_any_kernel<64, GROUPS>), grid, dim3(256), 0, s, a);
+  else if (a.D <= 96) hipLaunchKernelGGL((prompt_any_kernel<96, GROUPS>), grid, dim3(256), 0, s, a);
+  else if (a.D <= 128) hipLaunchKernelGGL((prompt_any_kernel<128, GROUPS>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((prompt_any_kernel<256, GROUPS>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
+}
+
+hipError_t launch_prompt_any(const PromptArgs& a, hipStream_t s) {
+  const long wgs = (long)a.n_tiles * a.H * (((long)a.tile_m * a.gqa + kRows - 1) / kRows);
+  return wgs <= (a.D <= 128 ? 3 * 256 : 256) ? launch_prompt_any_t<2>(a, s) : launch_prompt_any_t<1>(a, s);
 }
 
 hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s) {

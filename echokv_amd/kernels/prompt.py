@@ -8,7 +8,8 @@ same query rows over them (``kernels.shared.prefix_attention``) and its log-sum-
 reference has no counterpart: its prefill reads the chunk back from the cache
 (``echokv_vllm/kernels/prefill.py:170-207``).
 
-Kernels: ``echokv_amd/csrc/attend_any.hip``, through ``echokv_prompt``.
+Kernels: ``echokv_amd/csrc/prompt.hip`` (float16 and bfloat16 of head size 64, 128 or 256) and
+``echokv_amd/csrc/attend_any.hip`` (32-bit arithmetic, every other case), through ``echokv_prompt``.
 """
 
 from __future__ import annotations
@@ -83,7 +84,10 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     ``lse`` (float32 ``[T, Hq]``) receives each row's log-sum-exp of the scaled scores, in log2
     units. ``prefix = (part, part_lse)``: attention of the same rows over keys before their
     prompt, float32 ``[T, Hq, D]`` with its log-sum-exp ``[T, Hq]``
-    (``kernels.shared.prefix_attention``), joined with the result."""
+    (``kernels.shared.prefix_attention``), joined with the result; a row whose ``part_lse`` is -inf
+    has none. 16-bit rows of head size 64, 128 or 256 have the same bits whatever else the step
+    holds; in the 32-bit kernels (every other case) they depend on the step's size through float
+    rounding."""
     if plan is None and not prefill:
         return
     qs, ks = query.shape, key.shape

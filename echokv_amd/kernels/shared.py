@@ -10,8 +10,10 @@ takes vLLM's ``common_prefix_len`` and does not use it (``echokv_vllm/backend.py
 The prefix is cut into ranges by the number of query rows, so a sequence's result depends on
 its batch through float rounding (``decode_attention`` alone is batch-invariant).
 
-Kernels: ``echokv_amd/csrc/attend_any.hip``, through ``echokv_prefix`` and
-``echokv_shared_decode``.
+Kernels: ``echokv_amd/csrc/shared.hip`` (head sizes 64, 128 and 256; queries and keys there are
+float16 parts, so both are to stay within float16's range, as in ``decode_attention``), and
+``echokv_amd/csrc/attend_any.hip`` (32-bit arithmetic for every other layout, and the join), through
+``echokv_prefix`` and ``echokv_shared_decode``.
 """
 
 from __future__ import annotations
@@ -127,10 +129,11 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
 
     Arguments as ``decode_attention``'s; ``seq_lens[i]`` counts the prefix, and row
     ``bt_rows[i]`` of the block table begins with the shared blocks. ``blocks``: their list (int32), by
-    default the first row of the table. A sequence shorter than ``prefix_len`` (length 0:
-    graph padding) leaves its row untouched. ``num_splits`` and ``blocks_per_split`` (default
-    ``suffix_blocks``) cut the tokens behind the prefix. ``workspace``: uint8, ``shared_workspace_bytes(...)``; by default the
-    call allocates it. A prefix of 0 tokens is plain decode."""
+    default the first row of the table (name it where that row is padding). A sequence shorter than
+    ``prefix_len`` (length 0: graph padding) leaves its row untouched. ``num_splits`` and
+    ``blocks_per_split`` (default ``suffix_blocks``) cut the tokens behind the prefix.
+    ``workspace``: uint8, ``shared_workspace_bytes(...)``; by default the call allocates it. A prefix
+    of 0 tokens is plain decode."""
     prefix_len = int(prefix_len)
     if prefix_len == 0:
         return dec.decode_attention(store, query, block_table, seq_lens, softmax_scale,

@@ -60,6 +60,18 @@ def test_matches_float64(device, lens, h, gqa, d, dtype):
         assert (out[b : b + 3] == 7.0).all() and (lse[b : b + 3] == 7.0).all()
 
 
+@pytest.mark.parametrize("h,gqa,d,lens", [(8, 4, 96, [1500, 3, 70]), (8, 5, 20, [40] * 50), (2, 4, 256, [2100]),
+                                          (1, 160, 64, [300])])
+def test_many_workgroups_in_32_bits(device, h, gqa, d, lens):
+    """More than three workgroups of 64 rows a CU: each keeps all of its keys' steps."""
+    print(f"[prompt] many workgroups D{d}", flush=True)
+    q, k, v, entries = make(device, lens, h, gqa, d, F32, seed=71)
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device=device)
+    prompt_attention(q, k, v, out, entries, d ** -0.5, lse=lse)
+    torch.cuda.synchronize()
+    check_all(q, k, v, entries, out, lse, d ** -0.5)
+
+
 @pytest.mark.parametrize("n", [255, 256, 1023, 1500, 4099])
 def test_long_prompts(device, n):
     print(f"[prompt] one of {n}", flush=True)
