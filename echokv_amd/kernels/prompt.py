@@ -85,9 +85,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     units. ``prefix = (part, part_lse)``: attention of the same rows over keys before their
     prompt, float32 ``[T, Hq, D]`` with its log-sum-exp ``[T, Hq]``
     (``kernels.shared.prefix_attention``), joined with the result; a row whose ``part_lse`` is -inf
-    has none. 16-bit rows of head size 64, 128 or 256 have the same bits whatever else the step
-    holds; in the 32-bit kernels (every other case) they depend on the step's size through float
-    rounding."""
+    has none. 16-bit rows of head size 64, 128 or 256, 16-byte aligned, have the same bits whatever
+    else the step holds; in the 32-bit kernels (every other case) they depend on the step's size
+    through float rounding."""
     if plan is None and not prefill:
         return
     qs, ks = query.shape, key.shape
