@@ -787,6 +787,7 @@ int64_t echokv_shared_decode_workspace(const echokv_layout* L, int32_t num_q_hea
                                        int64_t prefix_len, int32_t num_splits) {
   if (!prefix_shape_ok(L, num_q_heads, num_seqs, prefix_len)) return -ECHOKV_ESHAPE;
   if (num_splits <= 0 || num_splits > (1 << 20)) return -ECHOKV_EINVAL;
+  if (num_seqs > INT32_MAX / L->num_kv_heads / num_splits) return -ECHOKV_ESHAPE;  // the decode's grid
   if (num_seqs == 0) return 0;
   const int64_t ranges = prefix_ranges(L, num_q_heads, num_seqs, prefix_len);
   return (num_seqs * 8 + 15) / 16 * 16 + pack_bytes(L, num_q_heads, num_seqs, prefix_len) +

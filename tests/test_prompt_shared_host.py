@@ -128,6 +128,7 @@ def test_prefix_entry_rejects_bad_arguments(lib):
 
 def test_shared_entry_rejects_bad_arguments(lib):
     for kw, code in ((dict(hq=30), 2), (dict(n=-1), 2), (dict(prefix=0), 1), (dict(prefix=63), 1), (dict(splits=0), 1),
+                     (dict(n=1 << 20, splits=1 << 20, bytes=1 << 62), 2),
                      (dict(splits=1 << 30), 1), (dict(bps=0), 1), (dict(tier=3), 1), (dict(dtype=5), 3), (dict(od=5), 3),
                      (dict(blocks=None), 1), (dict(out=None), 1), (dict(bytes=100), 1), (dict(ws=None), 1),
                      (dict(ws=C.c_void_p(8)), 1), (dict(n=0), 0)):
