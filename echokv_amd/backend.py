@@ -71,8 +71,8 @@ MAX_HEAD_SIZE = 256
 MAX_DECODE_SPLITS = dec.MAX_SPLITS
 # A shared prefix from this long on is attended to apart (ECHOKV_SHARED_PREFIX=1). Apart it costs
 # two launches more, and its keys are a chain of steps in either form: decode of 1 to 64 requests
-# of 100-400 tokens behind 512 takes 27-36 us plainly, 32-42 apart; behind 1024 40-58 and 33-44;
-# behind 8192 73-193 and 40-61 (INT4, 8 KV heads of GQA 4 or 2 of GQA 8).
+# of 100-400 tokens behind 512 takes 27-37 us plainly, 32-47 apart; behind 1024 40-57 and 33-49;
+# behind 8192 73-193 and 40-65 (INT4, 8 KV heads of GQA 4 or 2 of GQA 8).
 SHARED_PREFIX_TOKENS = 1024
 
 

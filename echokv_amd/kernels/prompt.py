@@ -59,11 +59,17 @@ def build_prompt_plan(prefill, gqa: int, head_size: int, device) -> PromptPlan:
     most keys first, so that the longest workgroups start earliest."""
     tile_m = _lib.size("echokv_prompt_tile_m", gqa, 1, head_size)
     entries = _entries(prefill)
-    rows = [(qs, qe - qs, t, min(tile_m, qe - qs - t)) for qs, qe in entries for t in range(0, qe - qs, tile_m)]
-    rows.sort(key=lambda r: -(r[2] + r[3]))
-    tiles = torch.from_numpy(np.array(rows, np.int32).reshape(-1, 4))
-    return PromptPlan(to_device(tiles, device), tile_m, max((qe for _, qe in entries), default=0), entries, gqa,
-                      head_size)
+    reach = max((qe for _, qe in entries), default=0)
+    if reach > np.iinfo(np.int32).max:
+        raise ValueError(f"the prompts reach row {reach}: rows are 32 bits")
+    start, end = np.array(entries, np.int64).reshape(-1, 2).T
+    n = -(-(end - start) // tile_m)  # tiles of each prompt
+    seq = np.repeat(np.arange(len(entries)), n)
+    first = (np.arange(seq.size) - np.repeat(np.cumsum(n) - n, n)) * tile_m
+    last = np.minimum(first + tile_m, (end - start)[seq])
+    rows = np.stack([start[seq], (end - start)[seq], first, last - first], 1)[np.argsort(-last, kind="stable")]
+    tiles = torch.from_numpy(rows.astype(np.int32))
+    return PromptPlan(to_device(tiles, device), tile_m, reach, entries, gqa, head_size)
 
 
 def _row_state(lse: torch.Tensor, rows: int, hq: int, name: str) -> torch.Tensor:

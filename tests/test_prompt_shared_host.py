@@ -45,7 +45,7 @@ def test_plan_covers_every_row_once(lib, gqa, d):
     assert keys == sorted(keys, reverse=True)
 
 
-@pytest.mark.parametrize("entries", [[(3, 2)], [(-1, 4)], [(0, 10), (5, 20)], [(0, 4), (0, 4)], [(0, 9), (2, 3)]])
+@pytest.mark.parametrize("entries", [[(3, 2)], [(0, 1 << 31)], [(-1, 4)], [(0, 10), (5, 20)], [(0, 4), (0, 4)], [(0, 9), (2, 3)]])
 def test_plan_refuses_bad_rows(lib, entries):
     with pytest.raises(ValueError):
         build_prompt_plan(entries, 4, 128, CPU)
