@@ -661,10 +661,11 @@ bool prefix_mfma(const echokv_layout* L) {
 }
 
 // Ranges of a shared prefix, at least 128 keys each: as many as keep the workgroups within the
-// chip's 256 CUs (one each). A second round of them costs more than it fills: 594 rows of GQA 4
-// behind 2048 keys (80 workgroups a range) take 87, 74 and 94 us in 2, 3 and 4 ranges, 64 of
-// GQA 4 behind 4096 (8 a range) 74, 63 and 61 in 8, 16 and 32, 256 of GQA 4 behind 16384 (32)
-// 317, 206 and 225 in 4, 8 and 16, 8065 rows behind 8192 (1008) 2001 and 2222 in 1 and 2.
+// chip's 256 CUs (one each). Fewer leave CUs idle, a second round of them costs more than it fills.
+// us a call for half / this / twice the workgroups, GQA 4, 8 KV heads, INT4: 1 row behind 4096 keys
+// 20.0 / 16.4 / 16.4, 64 behind 4096 30.8 / 29.5 / 29.5, 64 behind 16384 74 / 54 / 68, 256 behind
+// 16384 183 / 137 / 162, 594 behind 2048 78 / 60 / 70, 594 behind 8192 269 / 165 / 169, 2000 behind
+// 8192 401 / 402 / 445.
 int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
   const int64_t n_rows = n * (hq / L->num_kv_heads), rows = prefix_mfma(L) ? ek::prefix_rows(L->head_size, ECHOKV_F16, n_rows) : 64;
   const int64_t wgs = (n_rows + rows - 1) / rows * L->num_kv_heads;

@@ -418,7 +418,9 @@ struct PrefixArgs {
 constexpr int kPackKeys = 64;  // keys of a tile of the dequantized prefix
 inline int64_t prefix_pack_bytes(int H, int D, int64_t len) { return (len + kPackKeys - 1) / kPackKeys * H * (kPackKeys * D * 6); }
 // Query rows of a workgroup of the 16-bit kernel: 32 per wave, four waves or (16-bit queries up to
-// head size 128, more than 128 rows) eight.
+// head size 128, more than 128 rows) eight. us of a shared decode with four / eight, GQA 4, 8 KV
+// heads, INT4, suffixes of 100-300: 33 sequences behind 1024 38 / 39, 4096 49 / 50, 16384 87 / 72; 64
+// behind 1024 42 / 45, 4096 52 / 54, 16384 92 / 78.
 inline int prefix_rows(int head_size, int q_dtype, int64_t rows) {
   return head_size <= 128 && q_dtype != ECHOKV_F32 && rows > 128 ? 256 : 128;
 }
