@@ -660,21 +660,6 @@ bool prefix_mfma(const echokv_layout* L) {
          L->num_blocks * L->chunks_per_page < (1LL << 24);
 }
 
-// Ranges of a shared prefix, at least 128 keys each: as many as keep the workgroups within the
-// chip's 256 CUs (one each). Fewer leave CUs idle, a second round of them costs more than it fills.
-// us a call for half / this / twice the workgroups, GQA 4, 8 KV heads, INT4: 1 row behind 4096 keys
-// 20.0 / 16.4 / 16.4, 64 behind 4096 30.8 / 29.5 / 29.5, 64 behind 16384 74 / 54 / 68, 256 behind
-// 16384 183 / 137 / 162, 594 behind 2048 78 / 60 / 70, 594 behind 8192 269 / 165 / 169, 2000 behind
-// 8192 401 / 402 / 445.
-int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
-  const int64_t n_rows = n * (hq / L->num_kv_heads), rows = prefix_mfma(L) ? ek::prefix_rows(L->head_size, ECHOKV_F16, n_rows) : 64;
-  const int64_t wgs = (n_rows + rows - 1) / rows * L->num_kv_heads;
-  int64_t r = 256 / (wgs > 0 ? wgs : 1);
-  const int64_t most = len / 128;
-  r = r < most ? r : most;
-  return (int)(r < 1 ? 1 : r < 64 ? r : 64);
-}
-
 // Whether the prefix is dequantized into a workspace first (16-bit queries, head size 64 or 128):
 // from three tiles of 256 rows on, and 8192 keys times tiles, less than which a second launch
 // takes longer than it saves. us in one pass / in two, GQA 4, 8 KV heads, INT4: 3 tiles over 1024
@@ -683,6 +668,24 @@ int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
 bool prefix_packed(const echokv_layout* L, int hq, int q_dtype, int64_t n, int64_t len) {
   const int64_t tiles = (n * (hq / L->num_kv_heads) + 255) / 256;
   return prefix_mfma(L) && L->head_size <= 128 && q_dtype != ECHOKV_F32 && tiles >= 3 && tiles * len >= 8192;
+}
+
+// Ranges of a shared prefix, at least 128 keys each: as many as keep the workgroups within the
+// chip's 256 CUs (one each). Fewer leave CUs idle, a second round of them costs more than it fills.
+// us a call for half / this / twice the workgroups, GQA 4, 8 KV heads, INT4: 1 row behind 4096 keys
+// 20.0 / 16.4 / 16.4, 64 behind 4096 30.8 / 29.5 / 29.5, 64 behind 16384 74 / 54 / 68, 256 behind
+// 16384 183 / 137 / 162, 594 behind 2048 78 / 60 / 70, 594 behind 8192 269 / 165 / 169, 2000 behind
+// 8192 401 / 402 / 445.
+int prefix_ranges(const echokv_layout* L, int hq, int64_t n, int64_t len) {
+  const int64_t n_rows = n * (hq / L->num_kv_heads);
+  const int64_t rows = !prefix_mfma(L)                          ? 64
+                       : prefix_packed(L, hq, ECHOKV_F16, n, len) ? 256
+                                                                  : ek::prefix_rows(L->head_size, ECHOKV_F16, n_rows, len);
+  const int64_t wgs = (n_rows + rows - 1) / rows * L->num_kv_heads;
+  int64_t r = 256 / (wgs > 0 ? wgs : 1);
+  const int64_t most = len / 128;
+  r = r < most ? r : most;
+  return (int)(r < 1 ? 1 : r < 64 ? r : 64);
 }
 
 bool prefix_shape_ok(const echokv_layout* L, int hq, int64_t n, int64_t len) {

@@ -418,11 +418,15 @@ struct PrefixArgs {
 constexpr int kPackKeys = 64;  // keys of a tile of the dequantized prefix
 inline int64_t prefix_pack_bytes(int H, int D, int64_t len) { return (len + kPackKeys - 1) / kPackKeys * H * (kPackKeys * D * 6); }
 // Query rows of a workgroup of the 16-bit kernel: 32 per wave, four waves or (16-bit queries up to
-// head size 128, more than 128 rows) eight. us of a shared decode with four / eight, GQA 4, 8 KV
-// heads, INT4, suffixes of 100-300: 33 sequences behind 1024 38 / 39, 4096 49 / 50, 16384 87 / 72; 64
-// behind 1024 42 / 45, 4096 52 / 54, 16384 92 / 78.
-inline int prefix_rows(int head_size, int q_dtype, int64_t rows) {
-  return head_size <= 128 && q_dtype != ECHOKV_F32 && rows > 128 ? 256 : 128;
+// head size 128, more than 128 rows) eight, which dequantize a key for twice the rows, from 6144 keys
+// times tiles of 256 rows on: fewer are a short chain either way, which two smaller workgroups a CU
+// run through sooner. us of a shared decode with four / eight, GQA 4, 8 KV heads, INT4, suffixes of
+// 100-300 tokens: 64 sequences (256 rows) behind 1024 keys 42 / 45, 4096 53 / 55, 8192 66 / 63, 16384
+// 92 / 79; 100 (2 tiles) behind 1024 47 / 50, 2048 54 / 55, 4096 66 / 62; 180 (3) behind 1024 58 /
+// 59, 2048 70 / 67.
+inline int prefix_rows(int head_size, int q_dtype, int64_t rows, int64_t len) {
+  const bool eight = head_size <= 128 && q_dtype != ECHOKV_F32 && rows > 128 && (rows + 255) / 256 * len >= 6144;
+  return eight ? 256 : 128;
 }
 
 // The ranges of the prefix and, in decode, the splits of the suffixes, added and normalized.

@@ -484,7 +484,7 @@ static hipError_t launch_d(const PrefixArgs& a, hipStream_t s) {
   }
   if constexpr (D == 256) return launch_t<D, false, 4>(a, s);
   else if (a.pack) return launch_packed<D>(a, s);
-  else return prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa) == 256 ? launch_t<D, false, 8>(a, s) : launch_t<D, false, 4>(a, s);
+  else return prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa, a.len) == 256 ? launch_t<D, false, 8>(a, s) : launch_t<D, false, 4>(a, s);
 }
 
 hipError_t launch_prefix(const PrefixArgs& a, hipStream_t s) {
