@@ -53,7 +53,8 @@ def prefix_attention(store, query: torch.Tensor, blocks: torch.Tensor, prefix_le
                      part: torch.Tensor | None = None, lse: torch.Tensor | None = None,
                      workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of every row of ``query [T, Hq, D]`` over the first ``prefix_len`` cached tokens
-    of the block list ``blocks`` (int32 ``[>= ceil(prefix_len / block_size)]``), each read once.
+    of the block list ``blocks`` (int32 ``[>= ceil(prefix_len / block_size)]``), each read once
+    (the tokens of a block outside the cache count as zeros).
 
     Returns ``(part, lse)``: normalized float32 rows ``[T, Hq, D]`` and their log-sum-exp
     ``[T, Hq]`` in log2 units (zeros and -inf for an empty prefix), what

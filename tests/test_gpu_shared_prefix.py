@@ -270,6 +270,84 @@ def test_pages_past_32_bits(device, d, seqs, prefix):
         check(out[i : i + 1], Rows(q[i : i + 1], k, v, [c.lens[i]], c.d ** -0.5), **BOUND)
 
 
+@pytest.mark.parametrize("d,dtype,seqs,prefix", [(128, F16, 5, 512), (128, F32, 5, 512), (96, BF16, 5, 512),
+                                                 (128, BF16, 200, 4096), (256, F16, 5, 64)], ids=str)
+def test_odd_strides(device, d, dtype, seqs, prefix):
+    """Queries, outputs and parts whose rows are aligned to one element."""
+    print(f"[shared] odd strides {d} {dtype} {seqs}", flush=True)
+    c = Cache(device, prefix, [5] * seqs, d=d, vg=24 if d == 96 else 32)
+    q = c.queries(seqs, 4, dtype)
+
+    def odd(x, t):
+        y = torch.full((x.shape[0], x.shape[1] + 1, d + 3), 7.0, dtype=t, device=device)
+        return y, y[:, 1:, 1 : d + 1]
+
+    qw, qo = odd(q, dtype)
+    qo.copy_(q)
+    lens = torch.tensor(c.lens, device=device)
+    part, lse = prefix_attention(c.store, q, c.blocks, prefix, c.d ** -0.5)
+    pw, po = odd(q, F32)
+    prefix_attention(c.store, qo, c.blocks, prefix, c.d ** -0.5, part=po)
+    out = shared_prefix_decode(c.store, q, c.table, lens, prefix, c.d ** -0.5, out=torch.empty_like(q))
+    ow, oo = odd(q, dtype)
+    shared_prefix_decode(c.store, qo, c.table, lens, prefix, c.d ** -0.5, out=oo)
+    torch.cuda.synchronize()
+    assert torch.equal(po, part) and torch.equal(oo, out)
+    for w in (pw, ow):
+        assert (w[:, 0] == 7).all() and (w[:, 1:, 0] == 7).all() and (w[:, 1:, d + 1 :] == 7).all()
+
+
+@pytest.mark.parametrize("prefix", [64, 4096])
+def test_large_gqa(device, prefix):
+    """More query heads a KV head than a workgroup has rows."""
+    print(f"[shared] gqa 300, {prefix}", flush=True)
+    c = Cache(device, prefix, [30, 5], h=1)
+    q = c.queries(2, 300, F16)
+    part, lse = prefix_attention(c.store, q, c.blocks, prefix, c.d ** -0.5)
+    out = shared_prefix_decode(c.store, q, c.table, torch.tensor(c.lens, device=device), prefix, c.d ** -0.5)
+    torch.cuda.synchronize()
+    check_prefix(c, q, part, lse, prefix, c.d ** -0.5)
+    check_decode(c, q, out, c.lens, c.d ** -0.5)
+
+
+def test_two_streams_at_once(device):
+    """Calls on two streams side by side: each has a workspace of its own."""
+    print("[shared] two streams", flush=True)
+    c = Cache(device, 4096, [60, 33, 1, 90] * 16)
+    qs = [c.queries(64, 4, F16, seed=i) for i in range(2)]
+    lens = torch.tensor(c.lens, device=device)
+    alone = [shared_prefix_decode(c.store, q, c.table, lens, 4096, 0.088) for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in qs], [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(shared_prefix_decode(c.store, qs[i], c.table, lens, 4096, 0.088))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, alone[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("d,rows,prefix", [(128, 5, 500), (128, 60, 8192), (96, 5, 500), (128, 200, 4096)])
+def test_blocks_outside_the_cache_are_zeros(device, d, rows, prefix):
+    print(f"[shared] blocks outside {d} {rows}", flush=True)
+    c = Cache(device, prefix, [], d=d, vg=24 if d == 96 else 32)
+    q = c.queries(rows, 4, F16)
+    bad = {3: -1, 7: c.store.pages.shape[0], 20: 1 << 30}
+    blocks = c.blocks.clone()
+    for i, b in bad.items():
+        blocks[i] = b
+    part, lse = prefix_attention(c.store, q, blocks, prefix, c.d ** -0.5)
+    torch.cuda.synchronize()
+    k, v = c.tokens(0, prefix)
+    for i in bad:
+        k[i * c.bs : (i + 1) * c.bs] = 0
+        v[i * c.bs : (i + 1) * c.bs] = 0
+    r = Rows(q[:8], k, v, [prefix] * min(8, rows), c.d ** -0.5)
+    check(part[:8], r, **BOUND)
+    assert float((lse[:8].double() - r.lse).abs().max()) <= r.lse_bound(BOUND["operands"])
+
+
 def test_no_prefix_is_plain_decode(device):
     c = Cache(device, 0, [30, 5], bs=16)
     q = c.queries(2, 4, F16)
