@@ -338,13 +338,12 @@ __global__ __launch_bounds__(256) void prefix_any_kernel(PrefixArgs a) {
 }
 
 // One wave per (entry, query head): its prefix ranges, then its suffix splits, 64 pieces at a
-// time, a group of 8 rows requested while the one before is added (the kernel is a chain of
-// round trips to memory). 2048 rows of 32 ranges and up to 4 splits take 9.6 us (38 MB, 4.0 TB/s),
-// 19008 of 3 ranges 14.4 (40 MB, 2.8 TB/s). Lane l holds channels [C l, C l + C) where the head is 64 C channels
+// time, a group of rows requested while the one before is added (the kernel is a chain of
+// round trips to memory). 2048 rows of 16 ranges and up to 4 splits take 7.0 us (21 MB, 3.0 TB/s),
+// 19008 of 3 ranges 11 (40 MB, 3.6 TB/s). Lane l holds channels [C l, C l + C) where the head is 64 C channels
 // (ANY false: one vector load a piece), else l, l + 64, ...
-template <int C, bool ANY>
+template <int C, bool ANY, int GROUP>
 __global__ __launch_bounds__(256) void join_kernel(JoinArgs a) {
-  constexpr int GROUP = 8;
   typedef float vec_t __attribute__((ext_vector_type(C)));
   const int lane = threadIdx.x & 63;
   const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);  // entry * hq + head
@@ -453,14 +452,23 @@ hipError_t launch_prefix_any(const PrefixArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_join(const JoinArgs& a, hipStream_t s) {
+template <int GROUP>
+static hipError_t launch_join_t(const JoinArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)((a.n * a.hq + 3) / 4));
-  if (a.D == 64) hipLaunchKernelGGL((join_kernel<1, false>), grid, dim3(256), 0, s, a);
-  else if (a.D == 128) hipLaunchKernelGGL((join_kernel<2, false>), grid, dim3(256), 0, s, a);
-  else if (a.D == 256) hipLaunchKernelGGL((join_kernel<4, false>), grid, dim3(256), 0, s, a);
-  else if (a.D < 128) hipLaunchKernelGGL((join_kernel<2, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((join_kernel<4, true>), grid, dim3(256), 0, s, a);
+  if (a.D == 64) hipLaunchKernelGGL((join_kernel<1, false, GROUP>), grid, dim3(256), 0, s, a);
+  else if (a.D == 128) hipLaunchKernelGGL((join_kernel<2, false, GROUP>), grid, dim3(256), 0, s, a);
+  else if (a.D == 256) hipLaunchKernelGGL((join_kernel<4, false, GROUP>), grid, dim3(256), 0, s, a);
+  else if (a.D < 128) hipLaunchKernelGGL((join_kernel<2, true, GROUP>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<4, true, GROUP>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
+}
+
+// A group's rows past the last piece are that one again: up to four pieces are one group of four.
+// us of a prefix_attention in groups of eight / four: 594 rows of 3 ranges (behind 2048 keys) 60.2 /
+// 57.1, 900 of 2 (1024) 57.3 / 52.3, 1000 of 2 (2048) 80.8 / 76.3.
+hipError_t launch_join(const JoinArgs& a, hipStream_t s) {
+  const int most = a.ranges + (a.acc ? a.num_splits : 0);
+  return most <= 4 ? launch_join_t<4>(a, s) : launch_join_t<8>(a, s);
 }
 
 }  // namespace ek
