@@ -4,7 +4,10 @@
 // One workgroup per (32 query rows per wave, KV head, range of keys): rows are (entry, GQA head)
 // pairs, whatever sequence they belong to, so a key is dequantized once for all of them. Keys are
 // held as a float16 hi + lo pair (2^-22 of the value together) and values in float16 (one
-// rounding, as prefill.hip); each wave runs S^T, an online softmax and O^T over a step's keys
+// rounding, as prefill.hip). Weights are float16 for bfloat16 queries, whose outputs' rounding is
+// eight times theirs, and hi + lo for float16 and float32 ones (PLO): both roundings at once made
+// float16 outputs 1.6 times as far off as their own rounding does, values alone 1.3 times (the low
+// parts cost 1 to 7 % of a call). Each wave runs S^T, an online softmax and O^T over a step's keys
 // (tiles.h).
 //
 // prefix_kernel dequantizes each step into LDS itself: a thread takes items of four keys x eight
@@ -201,8 +204,8 @@ __device__ __forceinline__ Row row_of(const PrefixArgs& a, int h, int r) {
 }
 
 // The row's query as fragments: 16 bytes at a time, all requested together.
-template <int D, int NKB, bool QLO>
-__device__ __forceinline__ void load_query(Rows<D, false, NKB, 2, QLO>& w, const PrefixArgs& a, const Row& row, int hh) {
+template <int D, int NKB, bool QLO, bool PLO>
+__device__ __forceinline__ void load_query(Rows<D, false, NKB, 2, QLO, PLO>& w, const PrefixArgs& a, const Row& row, int hh) {
   constexpr int NS = D / 16, QW = QLO ? 2 : 1;
   w.set_scale(a.scale_log2);
   const uint8_t* src = (const uint8_t*)a.q + (row.q_row * a.q_s0 + (long)row.qh * a.q_s1 + 8 * hh) * (2 * QW);
@@ -244,8 +247,8 @@ __device__ __forceinline__ void mask_tail(f16v_t* s, int left, int hh) {
 }
 
 // The wave's rows out: range z's partial ones, or normalized ones with their log-sum-exp.
-template <int D, int NKB, bool QLO>
-__device__ __forceinline__ void write_rows(Rows<D, false, NKB, 2, QLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
+template <int D, int NKB, bool QLO, bool PLO>
+__device__ __forceinline__ void write_rows(Rows<D, false, NKB, 2, QLO, PLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
   const float l = halves_sum(w.l);
   asm volatile("" : "+v"(r));  // the row's place is found again, not kept through the loop
   const Row row = row_of(a, h, r);
@@ -279,7 +282,7 @@ __device__ __forceinline__ void write_suffix(const PrefixArgs& a) {
 
 }  // namespace
 
-template <int D, bool QLO, int WAVES>
+template <int D, bool QLO, int WAVES, bool PLO>
 __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) void prefix_kernel(PrefixArgs a) {
   static_assert(WAVES == 4 || WAVES == 8, "a thread takes its items' K and V, or one of them");
   constexpr bool BOTH = WAVES == 4;
@@ -310,7 +313,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
   }
   const int r = (tile * WAVES + wave) * 32 + j;
   const bool active = (tile * WAVES + wave) * 32 < (int)a.n * a.gqa;
-  Rows<D, false, NKB, 2, QLO> w;
+  Rows<D, false, NKB, 2, QLO, PLO> w;
   load_query(w, a, row_of(a, h, r), hh);
   w.clear();
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
       const int left = k_end - (k_begin + step * KEYS + sb);  // keys of this block that there are
       if (left <= 0) break;
       f16v_t s[NKB];
-      u4_t p[2 * NKB];
+      u4_t p[w.PW];
       w.template scores<SIDE>(k_lane + buf + sb * 2 * D, s);
       if (left < 32 * NKB) mask_tail<NKB>(s, left, hh);
       w.rescale(w.top(s));
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(256) void prefix_pack_kernel(PrefixArgs a) {
   it.store(a.pack + ((long)tile * a.L.H + h) * (3 * I::SIDE), 0, head, raw, true, true, true);
 }
 
-template <int D>
+template <int D, bool PLO>
 __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   constexpr int WAVES = 8, KEYS = kPackKeys, NKB = 2, SIDE = KEYS * D * 2;
   constexpr int KDMA = 2 * SIDE / 1024 / WAVES, VDMA = SIDE / 1024 / WAVES;
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   }
   const int r = (tile * WAVES + wave) * 32 + j;
   const bool active = (tile * WAVES + wave) * 32 < (int)a.n * a.gqa;
-  Rows<D, false, NKB, 2, false> w;
+  Rows<D, false, NKB, 2, false, PLO> w;
   load_query(w, a, row_of(a, h, r), hh);
   w.clear();
   const uint32_t k_lane = lds0 + k_at<D>(0, j, hh), v_lane = lds0 + V0 + v_at<D>(0, lane);
@@ -415,7 +418,7 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   auto body = [&](int step, f16v_t* cur, f16v_t* nxt) __attribute__((always_inline)) {
     advance(step);
     w.rescale(mt);
-    u4_t p[2 * NKB];
+    u4_t p[w.PW];
     w.template weights<true, SIDE>(cur, p, k_lane + (uint32_t)(((step + 1) & 1) * 2 * SIDE), nxt);
     mt = w.template values<true>(p, v_lane + (uint32_t)((step & 1) * SIDE), nxt);
     if (tail && step + 2 == n_steps) {
@@ -441,7 +444,7 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
     }
     advance(step);
     w.rescale(mt);
-    u4_t p[2 * NKB];
+    u4_t p[w.PW];
     w.template weights<false, SIDE>(s0, p, 0, s0);
     w.template values<false>(p, v_lane + (uint32_t)((step & 1) * SIDE), s0);
   } else {
@@ -450,41 +453,47 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   write_rows(w, a, h, r, z, hh);
 }
 
-template <int D, bool QLO, int WAVES>
+template <int D, bool QLO, int WAVES, bool PLO>
 static hipError_t launch_t(const PrefixArgs& a, hipStream_t s) {
   constexpr int lds = (WAVES == 8 ? 2 : 1) * 3 * 8192 * 2;
   static std::atomic<uint64_t> attr_done{0};
-  const hipError_t e = ensure_lds_limit((const void*)prefix_kernel<D, QLO, WAVES>, lds, &attr_done);
+  const hipError_t e = ensure_lds_limit((const void*)prefix_kernel<D, QLO, WAVES, PLO>, lds, &attr_done);
   if (e != hipSuccess) return e;
   constexpr int rows = 32 * WAVES;
   const dim3 grid((unsigned)((a.n * a.gqa + rows - 1) / rows * a.L.H), (unsigned)a.ranges);
-  hipLaunchKernelGGL((prefix_kernel<D, QLO, WAVES>), grid, dim3(64 * WAVES), lds, s, a);
+  hipLaunchKernelGGL((prefix_kernel<D, QLO, WAVES, PLO>), grid, dim3(64 * WAVES), lds, s, a);
   return hipGetLastError();
 }
 
-template <int D>
+template <int D, bool PLO>
 static hipError_t launch_packed(const PrefixArgs& a, hipStream_t s) {
   constexpr int lds = 6 * kPackKeys * D * 2;
   static std::atomic<uint64_t> attr_done{0};
-  hipError_t e = ensure_lds_limit((const void*)prefix_flash_kernel<D>, lds, &attr_done);
+  hipError_t e = ensure_lds_limit((const void*)prefix_flash_kernel<D, PLO>, lds, &attr_done);
   if (e != hipSuccess) return e;
   const unsigned packs = (unsigned)((a.len + kPackKeys - 1) / kPackKeys * a.L.H);
   hipLaunchKernelGGL(prefix_pack_kernel<D>, dim3(packs), dim3(256), 0, s, a);
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const dim3 grid((unsigned)((a.n * a.gqa + 255) / 256 * a.L.H), (unsigned)a.ranges);
-  hipLaunchKernelGGL(prefix_flash_kernel<D>, grid, dim3(512), lds, s, a);
+  hipLaunchKernelGGL((prefix_flash_kernel<D, PLO>), grid, dim3(512), lds, s, a);
   return hipGetLastError();
+}
+
+template <int D, bool PLO>
+static hipError_t launch_16(const PrefixArgs& a, hipStream_t s) {
+  if constexpr (D == 256) return launch_t<D, false, 4, PLO>(a, s);
+  else if (a.pack) return launch_packed<D, PLO>(a, s);
+  else if (prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa, a.len) == 256) return launch_t<D, false, 8, PLO>(a, s);
+  else return launch_t<D, false, 4, PLO>(a, s);
 }
 
 template <int D>
 static hipError_t launch_d(const PrefixArgs& a, hipStream_t s) {
   if (a.q_dtype == ECHOKV_F32) {
     if constexpr (D == 256) return hipErrorInvalidValue;  // its registers do not fit: attend_any.hip
-    else return launch_t<D, true, 4>(a, s);
+    else return launch_t<D, true, 4, true>(a, s);
   }
-  if constexpr (D == 256) return launch_t<D, false, 4>(a, s);
-  else if (a.pack) return launch_packed<D>(a, s);
-  else return prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa, a.len) == 256 ? launch_t<D, false, 8>(a, s) : launch_t<D, false, 4>(a, s);
+  return a.q_dtype == ECHOKV_F16 ? launch_16<D, true>(a, s) : launch_16<D, false>(a, s);
 }
 
 hipError_t launch_prefix(const PrefixArgs& a, hipStream_t s) {

@@ -111,11 +111,14 @@ __device__ __forceinline__ h8_t v_read(uint32_t at, int ks) {
 // go between the score products of step i + 1, whose maxima go between the value products of
 // step i. Scheduling fences hold that order.
 //
-// PARTS: keys as one matrix or as hi + lo, `side` bytes apart. QLO: the queries as hi + lo too.
-template <int D, bool BF, int NKB, int PARTS, bool QLO>
+// PARTS: keys as one matrix or as hi + lo, `side` bytes apart. QLO: the queries as hi + lo too, PLO:
+// the weights as float16 hi + lo.
+template <int D, bool BF, int NKB, int PARTS, bool QLO, bool PLO = false>
 struct Rows {
   static constexpr int NS = D / 16, NDB = D / 32;
   static constexpr int NP = 8 * NKB;  // pairs of scores a lane
+  static constexpr int NW = 2 * NKB;  // words of 16 keys' weights, their low parts behind them
+  static constexpr int PW = PLO ? 2 * NW : NW;
   static constexpr float kShift = BF ? 0.f : 6.f;  // float16 weights are 2^6 times the softmax's: small ones keep their bits
   static constexpr float kInf = __builtin_inff();
   h8_t q[NS], ql[QLO ? NS : 1];
@@ -200,6 +203,10 @@ struct Rows {
       sum[0] += x[n & 1][0];
       sum[1] += x[n & 1][1];
       p[n / 4][n % 4] = pack2<BF>(x[n & 1][0], x[n & 1][1]);
+      if constexpr (PLO) {
+        const h2_t hi = __builtin_bit_cast(h2_t, (uint32_t)p[n / 4][n % 4]);
+        p[NW + n / 4][n % 4] = pack2<false>(x[n & 1][0] - (float)hi[0], x[n & 1][1] - (float)hi[1]);
+      }
     };
     if constexpr (NEXT) {
 #pragma unroll
@@ -244,6 +251,7 @@ struct Rows {
     for (int u = 0; u < VU; ++u) {
       if (u + AHEAD < VU) f[(u + AHEAD) % RING] = load(u + AHEAD);
       acc[u % NDB] = mma<BF>(f[u % RING], __builtin_bit_cast(h8_t, p[u / NDB]), acc[u % NDB]);
+      if constexpr (PLO) acc[u % NDB] = mma<BF>(f[u % RING], __builtin_bit_cast(h8_t, p[NW + u / NDB]), acc[u % NDB]);
       if constexpr (NEXT) {
 #pragma unroll
         for (int n = u * NP / VU; n < (u + 1) * NP / VU; ++n)
