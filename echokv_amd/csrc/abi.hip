@@ -699,9 +699,25 @@ bool prefix_shape_ok(const echokv_layout* L, int hq, int64_t n, int64_t len) {
 // Float32 rows of `hq` heads and their (max, sum) pairs, behind one another.
 int64_t rows_bytes(int64_t rows, int D) { return rows * (D + 2) * 4; }
 
-// The dequantized prefix in front of them, where a call may use it (float32 queries do not).
+// Keys of a range, whole steps of either kernel.
+int range_keys(int64_t len, int ranges) { return (int)((len + ranges - 1) / ranges + 127) / 128 * 128; }
+
+// A slab of the dequantized prefix in front of them, where a call may use it (float32 queries do
+// not): keys of each range (0: none) and bytes.
+int slab_keys(const echokv_layout* L, int hq, int64_t n, int64_t len) {
+  if (!prefix_packed(L, hq, ECHOKV_F16, n, len)) return 0;
+  const int ranges = prefix_ranges(L, hq, n, len);
+  return ek::prefix_seg(L->num_kv_heads, L->head_size, ranges, range_keys(len, ranges));
+}
 int64_t pack_bytes(const echokv_layout* L, int hq, int64_t n, int64_t len) {
-  return prefix_packed(L, hq, ECHOKV_F16, n, len) ? ek::prefix_pack_bytes(L->num_kv_heads, L->head_size, len) : 0;
+  const int64_t keys = slab_keys(L, hq, n, len) * (int64_t)prefix_ranges(L, hq, n, len);
+  return keys / ek::kPackKeys * L->num_kv_heads * ek::prefix_tile_bytes(L->head_size);
+}
+
+// Whether the rows leave the prefix kernel normalized: one range, in one slab.
+bool prefix_direct(const echokv_layout* L, int hq, int64_t n, int64_t len) {
+  const int seg = slab_keys(L, hq, n, len);
+  return prefix_ranges(L, hq, n, len) == 1 && (seg == 0 || seg == range_keys(len, 1));
 }
 
 // The shared part of echokv_prefix and echokv_shared_decode; n > 0 and the shapes checked.
@@ -727,9 +743,11 @@ ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const i
   a.len = (int)len;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.ranges = ranges;
-  a.per = (int)((len + ranges - 1) / ranges + 127) / 128 * 128;
+  a.per = range_keys(len, ranges);
   const bool packed = prefix_packed(L, hq, q_dtype, n, len) && (uintptr_t)pages % 16 == 0;
   a.pack = packed ? (uint8_t*)workspace : nullptr;
+  a.seg = slab_keys(L, hq, n, len);
+  a.slab = 0;
   a.acc = (float*)((uint8_t*)workspace + pack_bytes(L, hq, n, len));
   a.ml = a.acc + ranges * n * hq * L->head_size;
   a.part = nullptr;
@@ -755,8 +773,8 @@ extern "C" {
 int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t n, int64_t prefix_len) {
   if (!prefix_shape_ok(L, num_q_heads, n, prefix_len)) return -ECHOKV_ESHAPE;
   if (n == 0) return 0;
-  const int64_t ranges = prefix_ranges(L, num_q_heads, n, prefix_len);
-  return pack_bytes(L, num_q_heads, n, prefix_len) + (ranges > 1 ? rows_bytes(ranges * n * num_q_heads, L->head_size) : 0);
+  const int64_t rows = prefix_direct(L, num_q_heads, n, prefix_len) ? 0 : prefix_ranges(L, num_q_heads, n, prefix_len);
+  return pack_bytes(L, num_q_heads, n, prefix_len) + rows_bytes(rows * n * num_q_heads, L->head_size);
 }
 
 int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res, const int64_t* res_group,
@@ -774,7 +792,7 @@ int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* b
   const int ranges = prefix_ranges(L, num_q_heads, n, prefix_len);
   ek::PrefixArgs a = prefix_args(L, pages, block_res, res_group, res, query, q_s0, q_s1, q_dtype, num_q_heads, q_rows,
                                  n, blocks, prefix_len, softmax_scale, ranges, workspace);
-  if (ranges == 1) {
+  if (prefix_direct(L, num_q_heads, n, prefix_len)) {
     a.part = part;
     a.p_s0 = p_s0;
     a.p_s1 = p_s1;

@@ -413,10 +413,21 @@ struct PrefixArgs {
   // (0: one chunk a page).
   int bs_shift, kg_shift;
   uint32_t kc_mul;
-  uint8_t* pack;  // nullable: the dequantized prefix, prefix_pack_bytes (16-bit queries, head size 64 or 128)
+  // Nullable: room for a slab of the dequantized prefix (16-bit queries, head size 64 or 128), `seg`
+  // keys of each range. Slab `slab` holds the keys from slab * seg on of each.
+  uint8_t* pack;
+  int seg, slab;
 };
-constexpr int kPackKeys = 64;  // keys of a tile of the dequantized prefix
-inline int64_t prefix_pack_bytes(int H, int D, int64_t len) { return (len + kPackKeys - 1) / kPackKeys * H * (kPackKeys * D * 6); }
+constexpr int kPackKeys = 64;               // keys of a tile of the dequantized prefix
+constexpr int64_t kPackBytes = 128ll << 20;  // the slab, at most: its size does not grow with the prefix
+inline int64_t prefix_tile_bytes(int D) { return (int64_t)kPackKeys * D * 6; }
+// Keys of each range in a slab: all `per` of them where they fit, else equal parts.
+inline int prefix_seg(int H, int D, int ranges, int per) {
+  const int64_t tiles = per / kPackKeys, fit = kPackBytes / (ranges * H * prefix_tile_bytes(D));
+  if (fit >= tiles) return per;
+  const int64_t slabs = fit > 0 ? (tiles + fit - 1) / fit : tiles;
+  return (int)((tiles + slabs - 1) / slabs) * kPackKeys;
+}
 // Query rows of a workgroup of the 16-bit kernel: 32 per wave, four waves or (16-bit queries up to
 // head size 128, more than 128 rows) eight, which dequantize a key for twice the rows, from 6144 keys
 // times tiles of 256 rows on: fewer are a short chain either way, which two smaller workgroups a CU

@@ -18,7 +18,9 @@
 // With many rows the same keys would be dequantized again for every 256 of them:
 // prefix_pack_kernel dequantizes the prefix once into a workspace, in 64-key tiles laid out as
 // LDS holds them, and prefix_flash_kernel streams those by direct global-to-LDS loads, the loop of
-// prompt.hip.
+// prompt.hip. The workspace holds 128 MiB of tiles at most; a longer prefix goes through it slab by
+// slab, each slab the next part of every range, and a row goes on from the unnormalized output,
+// maximum and sum that the slab before left in its workspace row.
 //
 // Measured (8 KV heads of GQA 4, D 128): 64 sequences (256 rows) behind 4096 INT4 keys 23 us in
 // prefix_kernel, of which 16 ranges' partial rows (17 MB) are 3 at the rate of a copy and the loads'
@@ -271,6 +273,26 @@ __device__ __forceinline__ void write_rows(Rows<D, false, NKB, 2, QLO, PLO>& w, 
   }
 }
 
+// The wave's rows as range z's partial ones in the workspace are: what write_rows left there.
+template <int D, int NKB, bool QLO, bool PLO>
+__device__ __forceinline__ void resume_rows(Rows<D, false, NKB, 2, QLO, PLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
+  const Row row = row_of(a, h, r);
+  if (!row.live) return;
+  const long pr = ((long)z * a.n + row.t) * a.hq + row.qh;
+  const float2 ml = *(const float2*)(a.ml + 2 * pr);
+  w.m = ml.x + w.kShift;
+  w.l = hh == 0 ? ml.y : 0.f;  // the half-waves' shares are added at the end
+  const float* src = a.acc + pr * D + 4 * hh;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f4_t x = *(const f4_any_t*)(src + 32 * db + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w.acc[db][4 * g + e] = x[e];
+    }
+}
+
 // Decode: the lengths behind the prefix, for the kernels that follow.
 __device__ __forceinline__ void write_suffix(const PrefixArgs& a) {
   if (!a.suffix) return;
@@ -358,13 +380,23 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
   write_rows(w, a, h, r, z, hh);
 }
 
-// One workgroup per (64-key tile, KV head): its K hi, K lo and V into the workspace.
+// Range z's keys: [begin, end).
+__device__ __forceinline__ int range_begin(const PrefixArgs& a, int z) { return z * a.per; }
+__device__ __forceinline__ int range_end(const PrefixArgs& a, int z) {
+  return z == a.ranges - 1 ? a.len : min(a.len, (z + 1) * a.per);
+}
+
+// One workgroup per (64-key tile of the slab, KV head): its K hi, K lo and V into the workspace. A
+// range's tiles of the slab lie behind one another.
 template <int D>
 __global__ __launch_bounds__(256) void prefix_pack_kernel(PrefixArgs a) {
   using I = Items<D, kPackKeys>;
   write_suffix(a);
   const int h = (int)(blockIdx.x % (unsigned)a.L.H), tile = (int)(blockIdx.x / (unsigned)a.L.H);
-  const I it(a, h, tile * kPackKeys, min(a.len, (tile + 1) * kPackKeys), (int)threadIdx.x);
+  const int tiles = a.seg / kPackKeys, z = tile / tiles;
+  const int begin = range_begin(a, z) + a.slab * a.seg + tile % tiles * kPackKeys, end = range_end(a, z);
+  if (begin >= end) return;
+  const I it(a, h, begin, end - begin < kPackKeys ? end : begin + kPackKeys, (int)threadIdx.x);
   if (4 * it.quad >= kPackKeys) return;  // head size 64: half of the threads
   Raw raw;
   const Head head = it.load_head(it.load_blk(0));
@@ -382,10 +414,12 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int j = lane & 31, hh = lane >> 5;
   const int h = (int)(blockIdx.x % (unsigned)a.L.H), tile = (int)(blockIdx.x / (unsigned)a.L.H), z = blockIdx.y;
-  const int k_begin = z * a.per, k_end = z == a.ranges - 1 ? a.len : min(a.len, k_begin + a.per);
+  const int k_begin = range_begin(a, z) + a.slab * a.seg, z_end = range_end(a, z);
+  const int k_end = z_end - k_begin < a.seg ? z_end : k_begin + a.seg;  // this slab's keys of the range
   const int n_steps = k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
+  if (a.slab > 0 && n_steps == 0) return;  // the rows are as the slabs before left them
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  const uint8_t* tiles = a.pack + ((long)(k_begin / KEYS) * a.L.H + h) * (3 * SIDE);
+  const uint8_t* tiles = a.pack + ((long)z * (a.seg / KEYS) * a.L.H + h) * (3 * SIDE);
   auto issue = [&](int step, bool val) __attribute__((always_inline)) {
     const int n = val ? VDMA : KDMA;
     const uint8_t* from = uniform_ptr(tiles + (long)step * a.L.H * (3 * SIDE) + (val ? 2 * SIDE : 0) + 1024 * n * wave);
@@ -403,6 +437,7 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   Rows<D, false, NKB, 2, false, PLO> w;
   load_query(w, a, row_of(a, h, r), hh);
   w.clear();
+  if (a.slab > 0) resume_rows<D>(w, a, h, r, z, hh);
   const uint32_t k_lane = lds0 + k_at<D>(0, j, hh), v_lane = lds0 + V0 + v_at<D>(0, lane);
 
   // As in prompt.hip: at `step` the keys of `step` + 1 and the values of `step` have landed.
@@ -471,12 +506,17 @@ static hipError_t launch_packed(const PrefixArgs& a, hipStream_t s) {
   static std::atomic<uint64_t> attr_done{0};
   hipError_t e = ensure_lds_limit((const void*)prefix_flash_kernel<D, PLO>, lds, &attr_done);
   if (e != hipSuccess) return e;
-  const unsigned packs = (unsigned)((a.len + kPackKeys - 1) / kPackKeys * a.L.H);
-  hipLaunchKernelGGL(prefix_pack_kernel<D>, dim3(packs), dim3(256), 0, s, a);
-  if ((e = hipGetLastError()) != hipSuccess) return e;
+  const unsigned packs = (unsigned)((long)a.ranges * (a.seg / kPackKeys) * a.L.H);
   const dim3 grid((unsigned)((a.n * a.gqa + 255) / 256 * a.L.H), (unsigned)a.ranges);
-  hipLaunchKernelGGL((prefix_flash_kernel<D, PLO>), grid, dim3(512), lds, s, a);
-  return hipGetLastError();
+  PrefixArgs b = a;
+  for (int from = 0; from < a.per; from += a.seg, ++b.slab) {
+    hipLaunchKernelGGL(prefix_pack_kernel<D>, dim3(packs), dim3(256), 0, s, b);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL((prefix_flash_kernel<D, PLO>), grid, dim3(512), lds, s, b);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    b.suffix = nullptr;  // written by the first
+  }
+  return hipSuccess;
 }
 
 template <int D, bool PLO>

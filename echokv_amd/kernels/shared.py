@@ -88,7 +88,8 @@ def prefix_attention(store, query: torch.Tensor, blocks: torch.Tensor, prefix_le
 
 
 def prefix_workspace_bytes(store, num_q_heads: int, num_rows: int, prefix_len: int) -> int:
-    """Workspace of a ``prefix_attention`` call."""
+    """Workspace of a ``prefix_attention`` call, of any query type: partial rows by the number of rows,
+    and at most 128 MiB for keys dequantized once for many rows, however long the prefix is."""
     return _lib.size("echokv_prefix_workspace", _lib.byref(store.abi), num_q_heads, num_rows, prefix_len)
 
 

@@ -300,7 +300,8 @@ int echokv_prompt(const void* query, int64_t q_s0, int64_t q_s1, const void* key
  * once for all of them: the first prefix_len tokens of the block list `blocks` (device int32,
  * ceil(prefix_len / block_size) entries). part (float32, row q_rows[i], strides p_s0 / p_s1) gets
  * the normalized rows and lse (float [rows, num_q_heads]) their log2-domain log-sum-exp (zeros
- * and -inf for prefix_len 0). workspace: echokv_prefix_workspace(...) bytes, 16-byte aligned.
+ * and -inf for prefix_len 0). workspace: echokv_prefix_workspace(...) bytes, 16-byte aligned; it
+ * serves every query type and grows with n, with prefix_len by 128 MiB at most.
  * Results depend on n through float rounding (the keys are cut into ranges by it).
  * No counterpart in the reference. */
 int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t n, int64_t prefix_len);
