@@ -50,6 +50,7 @@ from echokv_amd._vllm import (
     AttentionType,
     MultipleOf,
 )
+from echokv_amd._util import to_device
 from echokv_amd.canary import canary_kl, ring_view
 from echokv_amd.config import load_config, v_group_supported
 from echokv_amd.controller import SUPPORTED_BITS, LayerController
@@ -220,6 +221,7 @@ class PromptWork:
     rows: tuple  # the step's query rows [first, last) that hold them
     plan: pm.PromptPlan  # of the chunks, by rows from the first one on
     prefix: SharedPrefix | None = None
+    own: torch.Tensor | None = None  # with a prefix: their rows, from the first on (None: all of `rows`)
 
     def run(self, impl, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, out: torch.Tensor) -> None:
         a, b = self.rows
@@ -227,7 +229,8 @@ class PromptWork:
         k, v = (x.view(x.shape[0], impl.num_kv_heads, impl.head_size)[a:b] for x in (key, value))
         before = None
         if self.prefix is not None:
-            before = sh.prefix_attention(impl.store, q, self.prefix.blocks, self.prefix.tokens, impl.scale)
+            before = sh.prefix_attention(impl.store, q, self.prefix.blocks, self.prefix.tokens, impl.scale,
+                                         q_rows=self.own)
         pm.prompt_attention(q, k, v, o, (), impl.scale, plan=self.plan, prefix=before)
 
 
@@ -453,7 +456,10 @@ class EchoKVMetadataBuilder(AttentionMetadataBuilder):
             if mine:
                 first, last = min(a for a, _ in mine), max(b for _, b in mine)
                 plan = pm.build_prompt_plan([(a - first, b - first) for a, b in mine], self.gqa, head_size, self.device)
-                work.append(PromptWork((first, last), plan, prefix if before else None))
+                own = None
+                if before and sum(b - a for a, b in mine) < last - first:  # other requests' rows between them
+                    own = to_device(torch.cat([torch.arange(a - first, b - first) for a, b in mine]), self.device)
+                work.append(PromptWork((first, last), plan, prefix if before else None, own))
         rest = [c for c in chunks if c[2] - (c[1] - c[0]) not in (0, shared)]
         return work, rest
 

@@ -18,6 +18,8 @@ float16 parts, so both are to stay within float16's range, as in ``decode_attent
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from echokv_amd import _lib
@@ -51,10 +53,13 @@ def _workspace(workspace: torch.Tensor | None, need: int, device) -> torch.Tenso
 
 def prefix_attention(store, query: torch.Tensor, blocks: torch.Tensor, prefix_len: int, softmax_scale: float,
                      part: torch.Tensor | None = None, lse: torch.Tensor | None = None,
-                     workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                     workspace: torch.Tensor | None = None,
+                     q_rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of every row of ``query [T, Hq, D]`` over the first ``prefix_len`` cached tokens
     of the block list ``blocks`` (int32 ``[>= ceil(prefix_len / block_size)]``), each read once
-    (the tokens of a block outside the cache count as zeros).
+    (the tokens of a block outside the cache count as zeros). ``q_rows`` (int64 indices into
+    ``query``): of these rows alone; the others are left as they are, with a log-sum-exp of -inf where
+    the call allocates ``lse``.
 
     Returns ``(part, lse)``: normalized float32 rows ``[T, Hq, D]`` and their log-sum-exp
     ``[T, Hq]`` in log2 units (zeros and -inf for an empty prefix), what
@@ -63,15 +68,23 @@ def prefix_attention(store, query: torch.Tensor, blocks: torch.Tensor, prefix_le
     query = _query(store, query)
     t, hq, d = query.shape
     prefix_len = int(prefix_len)
-    need = prefix_workspace_bytes(store, hq, t, prefix_len)
-    _lib.require_current(query, blocks, part, lse, workspace, store.pages)
+    if q_rows is not None and q_rows.dim() != 1:
+        raise ValueError("q_rows must be one row index after another")
+    n = t if q_rows is None else q_rows.shape[0]
+    if n and not t:
+        raise ValueError(f"{n} row indices, no query rows")
+    need = prefix_workspace_bytes(store, hq, n, prefix_len)
+    _lib.require_current(query, blocks, part, lse, workspace, q_rows, store.pages)
     blocks = _blocks(store, blocks, prefix_len)
+    q_rows = dec._i64(q_rows, query.device)
     if part is None:
         part = torch.empty(t, hq, d, device=query.device, dtype=torch.float32)
     if part.dtype != torch.float32 or part.shape != query.shape or part.stride(2) != 1:
         raise ValueError(f"part must be float32 {tuple(query.shape)} with contiguous channels")
     if lse is None:
         lse = torch.empty(t, hq, device=query.device, dtype=torch.float32)
+        if q_rows is not None:
+            lse.fill_(-math.inf)
     if lse.dtype != torch.float32 or lse.shape != (t, hq) or not lse.is_contiguous():
         raise ValueError(f"lse must be contiguous float32 {(t, hq)}")
     ws = _workspace(workspace, need, query.device)
@@ -80,9 +93,9 @@ def prefix_attention(store, query: torch.Tensor, blocks: torch.Tensor, prefix_le
     p0, p1, _ = part.stride()
     _lib.call(
         "echokv_prefix", _lib.byref(store.abi), store.pages.data_ptr(), store.block_res.data_ptr(),
-        store.res_group.data_ptr(), _lib.byref(res), query.data_ptr(), q0, q1, _lib.dtype_code(query), hq, None, t,
-        blocks.data_ptr(), prefix_len, float(softmax_scale), _lib.ptr(ws), 0 if ws is None else ws.numel(),
-        part.data_ptr(), p0, p1, lse.data_ptr(), _lib.stream(),
+        store.res_group.data_ptr(), _lib.byref(res), query.data_ptr(), q0, q1, _lib.dtype_code(query), hq,
+        _lib.ptr(q_rows), n, blocks.data_ptr(), prefix_len, float(softmax_scale), _lib.ptr(ws),
+        0 if ws is None else ws.numel(), part.data_ptr(), p0, p1, lse.data_ptr(), _lib.stream(),
     )
     return part, lse
 

@@ -1,8 +1,9 @@
-"""CPU: how much workspace calls behind a shared prefix ask for."""
+"""CPU: how much workspace calls behind a shared prefix ask for, and which rows take part."""
 
 from types import SimpleNamespace
 
 import pytest
+import torch
 
 from echokv_amd import _lib
 from echokv_amd.kernels import shared as sh
@@ -41,3 +42,37 @@ def test_one_more_sequence_costs_about_one_more():
     s = store()
     a, b = (sh.shared_workspace_bytes(s, 32, n, 1 << 17, 4) for n in (128, 129))
     assert b - a <= 128 * MIB
+
+
+# ---- the backend's steps --------------------------------------------------------------------
+
+def _builder(monkeypatch):
+    from test_prompt_shared_host import _builder
+
+    return _builder(monkeypatch, ECHOKV_SHARED_PREFIX="1", ECHOKV_PROMPT_EXACT="1")
+
+
+def test_rows_of_other_requests_do_not_attend_to_the_prefix(monkeypatch):
+    """A chunk of a longer context between two prompts behind the prefix: only the prompts' rows."""
+    from echokv_amd.backend import SharedPrefix
+
+    b = _builder(monkeypatch)
+    prefix = SharedPrefix(1088, torch.zeros(17, dtype=torch.int32))
+    chunks = [(3, 8, 1093, 1), (8, 20, 9000, 2), (20, 23, 1091, 3)]
+    work, rest = b._prompt_work(chunks, prefix)
+    assert rest == [chunks[1]] and work[0].rows == (3, 23)
+    assert work[0].own.tolist() == [0, 1, 2, 3, 4, 17, 18, 19]
+    work, rest = b._prompt_work([(3, 8, 1093, 1), (8, 20, 1100, 2)], prefix)  # nothing between them
+    assert not rest and work[0].own is None
+
+
+def test_prefix_refuses_row_indices():
+    from echokv_amd.kernels.shared import prefix_attention
+
+    s = store(2)
+    s.pages, s.res_k = torch.zeros(1), None
+    blocks = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="row index"):
+        prefix_attention(s, torch.zeros(3, 8, 128), blocks, 64, 0.1, q_rows=torch.zeros(1, 3, dtype=torch.int64))
+    with pytest.raises(ValueError, match="no query rows"):
+        prefix_attention(s, torch.zeros(0, 8, 128), blocks, 64, 0.1, q_rows=torch.zeros(3, dtype=torch.int64))
