@@ -696,8 +696,9 @@ bool prefix_shape_ok(const echokv_layout* L, int hq, int64_t n, int64_t len) {
   return n >= 0 && n <= INT32_MAX / 64 / hq && len >= 0 && len <= INT32_MAX - 16384;
 }
 
-// Float32 rows of `hq` heads and their (max, sum) pairs, behind one another.
-int64_t rows_bytes(int64_t rows, int D) { return rows * (D + 2) * 4; }
+// Float32 rows of `hq` heads and their (max, sum) pairs, behind one another; what follows them is
+// aligned to 16 bytes, as its vector loads take it.
+int64_t rows_bytes(int64_t rows, int D) { return (rows * (D + 2) * 4 + 15) / 16 * 16; }
 
 // Keys of a range, whole steps of either kernel.
 int range_keys(int64_t len, int ranges) { return (int)((len + ranges - 1) / ranges + 127) / 128 * 128; }
@@ -813,7 +814,8 @@ int64_t echokv_shared_decode_workspace(const echokv_layout* L, int32_t num_q_hea
   if (num_seqs == 0) return 0;
   const int64_t ranges = prefix_ranges(L, num_q_heads, num_seqs, prefix_len);
   return (num_seqs * 8 + 15) / 16 * 16 + pack_bytes(L, num_q_heads, num_seqs, prefix_len) +
-         rows_bytes((ranges + num_splits) * num_seqs * num_q_heads, L->head_size);
+         rows_bytes(ranges * num_seqs * num_q_heads, L->head_size) +
+         rows_bytes(num_splits * num_seqs * num_q_heads, L->head_size);
 }
 
 int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,
@@ -840,7 +842,7 @@ int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int
   a.lens = seq_lens;
   a.suffix = suffix;
   if (run_prefix(L, a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;
-  float* acc = a.ml + ranges * num_seqs * num_q_heads * 2;
+  float* acc = (float*)((uint8_t*)a.acc + rows_bytes(ranges * num_seqs * num_q_heads, L->head_size));
   float* ml = acc + num_splits * num_seqs * num_q_heads * L->head_size;
   ek::JoinArgs j{a.acc, a.ml, ranges, nullptr, nullptr, suffix, num_splits, ek::Splits{}, seq_lens, (int)prefix_len,
                  L->block_size, q_rows, num_seqs, num_q_heads, L->head_size, out, o_s0, o_s1, out_dtype, nullptr};

@@ -8,7 +8,7 @@ import torch
 from attend64 import Rows, check, unit
 from test_gpu_backend import D, H, HQ, LAYERS, Batch, make_engine, run_layers, slots_for
 from test_gpu_shared_backend import BS, F16, PREFIX, cached, settings  # noqa: F401
-from test_gpu_shared_prefix import BF16, Cache, check_prefix
+from test_gpu_shared_prefix import BF16, BOUND, Cache, check_prefix
 
 from echokv_amd.kernels import shared as sh
 
@@ -35,6 +35,16 @@ def test_named_rows_alone(device, d, rows, prefix):
     assert (alone[1][rest] == float("-inf")).all()
     none = sh.prefix_attention(c.store, q, c.blocks, prefix, d ** -0.5, part=part, q_rows=index[:0])
     assert (none[1] == float("-inf")).all() and (part[rest] == 7).all()
+
+
+def test_an_odd_number_of_partial_rows(device):
+    """Head size 256, one sequence of 7 heads behind 5 ranges: the suffix's rows come behind 35 pairs."""
+    print("[rows] odd pairs", flush=True)
+    c = Cache(device, 640, [40], h=1, d=256)
+    q = c.queries(1, 7, F16)
+    out = sh.shared_prefix_decode(c.store, q, c.table, torch.tensor(c.lens, device=device), 640, 0.06)
+    torch.cuda.synchronize()
+    check(out, Rows(q, *c.tokens(0, c.lens[0]), [c.lens[0]], 0.06), **BOUND)
 
 
 def test_another_chunk_between_the_prompts(device, settings, monkeypatch):  # noqa: F811

@@ -44,6 +44,16 @@ def test_one_more_sequence_costs_about_one_more():
     assert b - a <= 128 * MIB
 
 
+@pytest.mark.parametrize("h,gqa,seqs,tokens,ranges", [(1, 7, 1, 640, 5), (1, 1, 1, 128, 1), (2, 4, 3, 640, 5)])
+def test_suffix_rows_are_aligned(h, gqa, seqs, tokens, ranges):
+    """The suffixes' rows, read by 16-byte loads, lie behind the prefix's (max, sum) pairs: an odd number
+    of those (5 ranges of 7 heads) is followed by 8 bytes of nothing."""
+    s, rows, splits, d = store(h, 256), seqs * h * gqa, 4, 256
+    size = sh.shared_workspace_bytes(s, h * gqa, seqs, tokens, splits)
+    lengths, pairs = -(-seqs * 8 // 16) * 16, -(-ranges * rows * 8 // 16) * 16
+    assert size == lengths + ranges * rows * d * 4 + pairs + splits * rows * d * 4 + splits * rows * 8
+
+
 # ---- the backend's steps --------------------------------------------------------------------
 
 def _builder(monkeypatch):
