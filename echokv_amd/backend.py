@@ -433,18 +433,25 @@ class EchoKVMetadataBuilder(AttentionMetadataBuilder):
                                    workspace=group.impls[0].decode_workspace(n_dec, self.num_splits, self.cap),
                                    batch_invariant=self.cfg.batch_invariant)
             if prefix is not None:
-                md.decode.prefix = self._decode_prefix(group, prefix, n_dec, int(lens.max()))
+                # The longest single-token request: a chunk in the step has no part in the decode.
+                longest = int(lens.numpy()[qsl[1:] - qsl[:-1] <= 1].max(initial=0))
+                md.decode.prefix = self._decode_prefix(group, prefix, n_dec, longest, md.decode.workspace)
         if up.prefill:
             md.prefill = self._prefill_work(group, up.prefill, prefix)
         return md
 
-    def _decode_prefix(self, group: _Group, prefix: SharedPrefix, n_dec: int, longest: int) -> SharedPrefix:
-        """``prefix`` with the splits and the workspace of the step's decode."""
+    def _decode_prefix(self, group: _Group, prefix: SharedPrefix, n_dec: int, longest: int,
+                       reserved: tuple | None) -> SharedPrefix:
+        """``prefix`` with the splits and the workspace of the step's decode: the one reserved for
+        plain decode, which this step does not run, where it is large enough."""
         store, hq = group.impls[0].store, group.impls[0].num_heads
         bs = self.kv_cache_spec.block_size
         splits = sh.suffix_splits(-(-longest // bs), bs, prefix.tokens, sh.suffix_blocks(store, n_dec), longest)
         need = sh.shared_workspace_bytes(store, hq, n_dec, prefix.tokens, splits)
-        return replace(prefix, num_splits=splits, workspace=torch.empty(need, dtype=torch.uint8, device=self.device))
+        ws = reserved[0].view(-1).view(torch.uint8) if reserved is not None else None
+        if ws is None or ws.numel() < need:
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return replace(prefix, num_splits=splits, workspace=ws)
 
     def _prompt_work(self, chunks: list, prefix: SharedPrefix | None) -> tuple[list, list]:
         """(the chunks that read this step's keys as ``PromptWork``, the other chunks)."""

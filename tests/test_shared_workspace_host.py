@@ -86,3 +86,49 @@ def test_prefix_refuses_row_indices():
         prefix_attention(s, torch.zeros(3, 8, 128), blocks, 64, 0.1, q_rows=torch.zeros(1, 3, dtype=torch.int64))
     with pytest.raises(ValueError, match="no query rows"):
         prefix_attention(s, torch.zeros(0, 8, 128), blocks, 64, 0.1, q_rows=torch.zeros(3, dtype=torch.int64))
+
+
+def test_decode_takes_the_reserved_workspace_and_its_own_lengths(monkeypatch):
+    """The plain decode's workspace where it is large enough, else memory of the step's own; the
+    splits by the sequences that decode."""
+    b = _builder(monkeypatch)
+    s = store(2, bs=64, kg=32)
+    group = SimpleNamespace(impls=[SimpleNamespace(store=s, num_heads=8)])
+    from echokv_amd.backend import SharedPrefix
+
+    prefix = SharedPrefix(1088, torch.zeros(17, dtype=torch.int32))
+    need = sh.shared_workspace_bytes(s, 8, 3, 1088, 4)
+    acc = torch.zeros(-(-need // (8 * 128 * 4)), 8, 128)
+    got = b._decode_prefix(group, prefix, 3, 1300, (acc, None))
+    assert got.num_splits == 4 and got.workspace.data_ptr() == acc.data_ptr() and got.workspace.numel() >= need
+    for reserved in (None, (acc[:1], None)):
+        got = b._decode_prefix(group, prefix, 3, 1300, reserved)
+        assert got.workspace.data_ptr() != acc.data_ptr() and got.workspace.numel() == need
+
+
+@pytest.mark.parametrize("chunk", [0, 3000])
+def test_a_chunk_does_not_cut_the_decode(monkeypatch, chunk):
+    """Two decodes of 1300 tokens, and a step that also prefills a request of 3000."""
+    import numpy as np
+
+    from echokv_amd import backend
+
+    b = _builder(monkeypatch)
+    n = 3 if chunk else 2
+    starts = np.array([0, 1, 2, 202][: n + 1], np.int32)
+    lens = torch.tensor([1300, 1290, chunk][:n])
+    asked = []
+    up = SimpleNamespace(decode=(torch.zeros(2),) * 3, prefill=[], tok=None, fin=None, fin_count=None, n_tokens=0, n_fin=0,
+                         canary_rows=None, n_canary=0, canary_ctx=None, tier_masks=None, host_tier_masks=None)
+    impl = SimpleNamespace(decode_workspace=lambda *a: None)
+    group = SimpleNamespace(impls=[impl], driver=SimpleNamespace(run=lambda *a: up, apply=lambda *a: None), tiers=lambda: [4],
+                            headers=None)
+    monkeypatch.setattr(b, "_bound", lambda: group)
+    monkeypatch.setattr(b, "_mapping", lambda cm, dummy: (lens, torch.zeros(int(starts[-1]), dtype=torch.int64)))
+    monkeypatch.setattr(b, "_decode_prefix", lambda g, p, n_dec, longest, ws: asked.append((n_dec, longest)))
+    monkeypatch.setattr(backend, "is_dummy_step", lambda cm: False)
+    cm = SimpleNamespace(num_reqs=n, num_actual_tokens=int(starts[-1]), causal=True, slot_mapping=None,
+                         query_start_loc_cpu=torch.from_numpy(starts),
+                         block_table_tensor=torch.zeros(n, 60, dtype=torch.int32))
+    b.build(1088, cm)
+    assert asked == [(2, 1300)]
