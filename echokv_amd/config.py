@@ -140,7 +140,8 @@ ATTENTION_SETTINGS: tuple[Setting, ...] = (
     Setting("ECHOKV_PROMPT_EXACT", "prompt_exact", _flag, lambda s: False),
     # Cached blocks that every request of a step begins with are attended to once for the batch
     # (vLLM's cascade attention); a request's result then depends on its batch through float
-    # rounding.
+    # rounding, and in bfloat16 models the prefix's weights and values are rounded to float16 in
+    # decode (2^-10 of weight x |value| at most; plain decode holds both exactly).
     Setting("ECHOKV_SHARED_PREFIX", "shared_prefix", _flag, lambda s: False),
 )
 

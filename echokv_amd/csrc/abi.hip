@@ -705,28 +705,38 @@ int range_keys(int64_t len, int ranges) { return (int)((len + ranges - 1) / rang
 
 // A slab of the dequantized prefix in front of them, where a call may use it (float32 queries do
 // not): keys of each range (0: none) and bytes.
-int slab_keys(const echokv_layout* L, int hq, int64_t n, int64_t len) {
+int slab_keys(const echokv_layout* L, int hq, int64_t n, int64_t len, bool exact) {
   if (!prefix_packed(L, hq, ECHOKV_F16, n, len)) return 0;
   const int ranges = prefix_ranges(L, hq, n, len);
-  return ek::prefix_seg(L->num_kv_heads, L->head_size, ranges, range_keys(len, ranges));
+  return ek::prefix_seg(L->num_kv_heads, L->head_size, exact, ranges, range_keys(len, ranges));
 }
-int64_t pack_bytes(const echokv_layout* L, int hq, int64_t n, int64_t len) {
-  const int64_t keys = slab_keys(L, hq, n, len) * (int64_t)prefix_ranges(L, hq, n, len);
-  return keys / ek::kPackKeys * L->num_kv_heads * ek::prefix_tile_bytes(L->head_size);
+int64_t slab_bytes(const echokv_layout* L, int hq, int64_t n, int64_t len, bool exact) {
+  const int64_t keys = slab_keys(L, hq, n, len, exact) * (int64_t)prefix_ranges(L, hq, n, len);
+  return keys / ek::kPackKeys * L->num_kv_heads * ek::prefix_tile_bytes(L->head_size, exact);
+}
+// What a workspace holds of it: a decode's for every type of its outputs.
+int64_t pack_bytes(const echokv_layout* L, int hq, int64_t n, int64_t len, bool decode) {
+  const int64_t one = slab_bytes(L, hq, n, len, false), two = decode ? slab_bytes(L, hq, n, len, true) : 0;
+  return one > two ? one : two;
 }
 
 // Whether the rows leave the prefix kernel normalized: one range, in one slab.
 bool prefix_direct(const echokv_layout* L, int hq, int64_t n, int64_t len) {
-  const int seg = slab_keys(L, hq, n, len);
+  const int seg = slab_keys(L, hq, n, len, false);
   return prefix_ranges(L, hq, n, len) == 1 && (seg == 0 || seg == range_keys(len, 1));
 }
 
-// The shared part of echokv_prefix and echokv_shared_decode; n > 0 and the shapes checked.
+// The shared part of echokv_prefix and echokv_shared_decode (out_dtype: its outputs', -1: no decode);
+// n > 0 and the shapes checked. A decode holds what the paged decode it stands for holds, weights and
+// values as exact float16 parts, where its outputs can show it: one rounding of each is an eighth of a
+// bfloat16 output's own, and up to twice a float16 one's.
 ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res,
                            const int64_t* res_group, const echokv_residual* res, const void* query, int64_t q_s0,
                            int64_t q_s1, int32_t q_dtype, int32_t hq, const int64_t* q_rows, int64_t n,
-                           const int32_t* blocks, int64_t len, float softmax_scale, int ranges, void* workspace) {
+                           const int32_t* blocks, int64_t len, float softmax_scale, int ranges, void* workspace,
+                           int32_t out_dtype) {
   ek::PrefixArgs a;
+  a.exact = out_dtype == ECHOKV_F16 || out_dtype == ECHOKV_F32;
   a.L = to_lay(L);
   a.pages = pages;
   a.block_res = block_res;
@@ -747,9 +757,9 @@ ek::PrefixArgs prefix_args(const echokv_layout* L, const uint8_t* pages, const i
   a.per = range_keys(len, ranges);
   const bool packed = prefix_packed(L, hq, q_dtype, n, len) && (uintptr_t)pages % 16 == 0;
   a.pack = packed ? (uint8_t*)workspace : nullptr;
-  a.seg = slab_keys(L, hq, n, len);
+  a.seg = slab_keys(L, hq, n, len, a.exact);
   a.slab = 0;
-  a.acc = (float*)((uint8_t*)workspace + pack_bytes(L, hq, n, len));
+  a.acc = (float*)((uint8_t*)workspace + pack_bytes(L, hq, n, len, out_dtype >= 0));
   a.ml = a.acc + ranges * n * hq * L->head_size;
   a.part = nullptr;
   a.p_s0 = a.p_s1 = 0;
@@ -775,7 +785,7 @@ int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int
   if (!prefix_shape_ok(L, num_q_heads, n, prefix_len)) return -ECHOKV_ESHAPE;
   if (n == 0) return 0;
   const int64_t rows = prefix_direct(L, num_q_heads, n, prefix_len) ? 0 : prefix_ranges(L, num_q_heads, n, prefix_len);
-  return pack_bytes(L, num_q_heads, n, prefix_len) + rows_bytes(rows * n * num_q_heads, L->head_size);
+  return pack_bytes(L, num_q_heads, n, prefix_len, false) + rows_bytes(rows * n * num_q_heads, L->head_size);
 }
 
 int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* block_res, const int64_t* res_group,
@@ -792,7 +802,7 @@ int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* b
   if (need > 0 && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return ECHOKV_EINVAL;
   const int ranges = prefix_ranges(L, num_q_heads, n, prefix_len);
   ek::PrefixArgs a = prefix_args(L, pages, block_res, res_group, res, query, q_s0, q_s1, q_dtype, num_q_heads, q_rows,
-                                 n, blocks, prefix_len, softmax_scale, ranges, workspace);
+                                 n, blocks, prefix_len, softmax_scale, ranges, workspace, -1);
   if (prefix_direct(L, num_q_heads, n, prefix_len)) {
     a.part = part;
     a.p_s0 = p_s0;
@@ -813,7 +823,7 @@ int64_t echokv_shared_decode_workspace(const echokv_layout* L, int32_t num_q_hea
   if (num_seqs > INT32_MAX / L->num_kv_heads / num_splits) return -ECHOKV_ESHAPE;  // the decode's grid
   if (num_seqs == 0) return 0;
   const int64_t ranges = prefix_ranges(L, num_q_heads, num_seqs, prefix_len);
-  return (num_seqs * 8 + 15) / 16 * 16 + pack_bytes(L, num_q_heads, num_seqs, prefix_len) +
+  return (num_seqs * 8 + 15) / 16 * 16 + pack_bytes(L, num_q_heads, num_seqs, prefix_len, true) +
          rows_bytes(ranges * num_seqs * num_q_heads, L->head_size) +
          rows_bytes(num_splits * num_seqs * num_q_heads, L->head_size);
 }
@@ -838,7 +848,7 @@ int echokv_shared_decode(const echokv_layout* L, const uint8_t* pages, const int
   int64_t* suffix = (int64_t*)workspace;
   float* rows = (float*)((uint8_t*)workspace + (num_seqs * 8 + 15) / 16 * 16);
   ek::PrefixArgs a = prefix_args(L, pages, block_res, res_group, res, query, q_s0, q_s1, q_dtype, num_q_heads, q_rows,
-                                 num_seqs, blocks, prefix_len, softmax_scale, ranges, rows);
+                                 num_seqs, blocks, prefix_len, softmax_scale, ranges, rows, out_dtype);
   a.lens = seq_lens;
   a.suffix = suffix;
   if (run_prefix(L, a, (hipStream_t)stream) != hipSuccess) return ECHOKV_ELAUNCH;

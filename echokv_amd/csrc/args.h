@@ -417,13 +417,15 @@ struct PrefixArgs {
   // keys of each range. Slab `slab` holds the keys from slab * seg on of each.
   uint8_t* pack;
   int seg, slab;
+  bool exact;  // decode into float16 or float32: weights and values as two float16 parts, as the paged decode
 };
 constexpr int kPackKeys = 64;               // keys of a tile of the dequantized prefix
 constexpr int64_t kPackBytes = 128ll << 20;  // the slab, at most: its size does not grow with the prefix
-inline int64_t prefix_tile_bytes(int D) { return (int64_t)kPackKeys * D * 6; }
+// K hi, K lo and V, or V hi and V lo.
+inline int64_t prefix_tile_bytes(int D, bool exact) { return (int64_t)kPackKeys * D * (exact ? 8 : 6); }
 // Keys of each range in a slab: all `per` of them where they fit, else equal parts.
-inline int prefix_seg(int H, int D, int ranges, int per) {
-  const int64_t tiles = per / kPackKeys, fit = kPackBytes / (ranges * H * prefix_tile_bytes(D));
+inline int prefix_seg(int H, int D, bool exact, int ranges, int per) {
+  const int64_t tiles = per / kPackKeys, fit = kPackBytes / (ranges * H * prefix_tile_bytes(D, exact));
   if (fit >= tiles) return per;
   const int64_t slabs = fit > 0 ? (tiles + fit - 1) / fit : tiles;
   return (int)((tiles + slabs - 1) / slabs) * kPackKeys;

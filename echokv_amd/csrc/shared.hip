@@ -3,12 +3,18 @@
 //
 // One workgroup per (32 query rows per wave, KV head, range of keys): rows are (entry, GQA head)
 // pairs, whatever sequence they belong to, so a key is dequantized once for all of them. Keys are
-// held as a float16 hi + lo pair (2^-22 of the value together) and values in float16 (one
-// rounding, as prefill.hip). Weights are float16 for bfloat16 queries, whose outputs' rounding is
-// eight times theirs, and hi + lo for float16 and float32 ones (PLO): both roundings at once made
-// float16 outputs 1.6 times as far off as their own rounding does, values alone 1.3 times (the low
-// parts cost 1 to 7 % of a call). Each wave runs S^T, an online softmax and O^T over a step's keys
-// (tiles.h).
+// held as a float16 hi + lo pair (2^-22 of the value together). Each wave runs S^T, an online softmax
+// and O^T over a step's keys (tiles.h).
+//
+// Decode into float16 or float32 holds weights and values as hi + lo pairs too (PLO, VLO), what the
+// paged decode it stands for holds: a float16 rounding of each is 2^-11 of weight x |value|, more than
+// 2e-3 where outlier channels reach 40. Into bfloat16, whose own rounding is eight times that, both are
+// float16. us a decode with one part / two: 4 sequences behind 512 28.7 / 29.9, 64 behind 4096 (GQA 4,
+// INT4) 63.9 / 65.3, 24 behind 8192 (GQA 8, INT2) 58.5 / 62.5, 256 behind 16384 (INT8) 204 / 258.
+// Prompts behind a prefix (float32 rows for prompt.hip to join) take values in float16, one rounding,
+// as prefill.hip, and weights in float16 for bfloat16 queries, hi + lo for float16 and float32 ones:
+// both roundings at once made float16 outputs 1.6 times as far off as their own rounding does, values
+// alone 1.3 times (the low parts cost 1 to 7 % of a call).
 //
 // prefix_kernel dequantizes each step into LDS itself: a thread takes items of four keys x eight
 // channels, of K in the first four waves and of V in the others (four waves: of both), its loads a
@@ -54,9 +60,10 @@ struct Head {
 // Items of the keys [k_begin, k_end) of head h in steps of KEYS: a thread's item of a step is four
 // keys x eight channels. Nothing loaded is looked at before the step that needs it, and no load
 // sits in a branch (addresses are clamped instead): the wave would wait for it there.
-template <int D, int KEYS>
+template <int D, int KEYS, bool VLO>
 struct Items {
-  static constexpr int OCTS = D / 8, SIDE = KEYS * D * 2;  // bytes of a step's K hi, K lo or V
+  static constexpr int OCTS = D / 8, SIDE = KEYS * D * 2;  // bytes of a step's K hi, K lo or V (VLO: V hi, V lo)
+  static constexpr int STEP = (VLO ? 4 : 3) * SIDE;
   const PrefixArgs& a;
   const int h, k_begin, k_end, oct, quad;
 
@@ -114,7 +121,8 @@ struct Items {
       }
     }
   }
-  __device__ __forceinline__ void put_k(uint8_t* buf, int i, const float* x8) const {
+  // Eight channels as float16 hi + lo, at `buf` + `at` and SIDE behind it.
+  __device__ __forceinline__ void put2(uint8_t* buf, int at, const float* x8) const {
     u4_t hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -122,16 +130,20 @@ struct Items {
       hi[e] = __builtin_bit_cast(uint32_t, p);
       lo[e] = pack2<false>(x8[2 * e] - (float)p[0], x8[2 * e + 1] - (float)p[1]);
     }
-    const int k = 4 * quad + i, at = k * (2 * D) + 16 * (oct ^ k_swz<D>(k));
     *(u4_t*)(buf + at) = hi;
     *(u4_t*)(buf + SIDE + at) = lo;
   }
-  __device__ __forceinline__ void put_v(uint8_t* buf, int i, const u4_t x) const {
+  __device__ __forceinline__ void put_k(uint8_t* buf, int i, const float* x8) const {
     const int k = 4 * quad + i;
-    *(u4_t*)(buf + 2 * SIDE + k * (2 * D) + 16 * (oct ^ v_swz<D>(k))) = x;
+    put2(buf, k * (2 * D) + 16 * (oct ^ k_swz<D>(k)), x8);
   }
-  // The item dequantized into a step's K hi, K lo and V at `buf` (LDS or memory; keys past the
-  // range and blocks that cannot be read: zeros).
+  __device__ __forceinline__ int v_slot(int i) const {
+    const int k = 4 * quad + i;
+    return k * (2 * D) + 16 * (oct ^ v_swz<D>(k));
+  }
+  __device__ __forceinline__ void put_v(uint8_t* buf, int i, const u4_t x) const { *(u4_t*)(buf + 2 * SIDE + v_slot(i)) = x; }
+  // The item dequantized into a step's sides at `buf` (LDS or memory; keys past the range and
+  // blocks that cannot be read: zeros).
   __device__ __forceinline__ void store(uint8_t* buf, int step, const Head& x, const Raw& w, bool keys, bool values,
                                         bool both) const {
     const Lay& L = a.L;
@@ -159,10 +171,17 @@ struct Items {
           h2_t c[4];
           code_pairs<B>((both ? w.v : w.k)[i], sh, c);
           const h2_t vs = u2h(w.vs[i] * 0x10001u), vm = u2h(w.vm[i] * 0x10001u);
-          u4_t v;
+          if constexpr (VLO) {
+            float x8[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[e], vs, vm));
-          put_v(buf, i, v);
+            for (int e = 0; e < 8; ++e) x8[e] = __builtin_fmaf((float)c[e >> 1][e & 1], (float)vs[0], (float)vm[0]);
+            put2(buf + 2 * SIDE, v_slot(i), x8);
+          } else {
+            u4_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[e], vs, vm));
+            put_v(buf, i, v);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -177,6 +196,7 @@ struct Items {
       for (int i = n_live > 0 ? n_live : 0; i < 4; ++i) {
         if (keys) put_k(buf, i, z8);
         if (values) put_v(buf, i, u4_t{});
+        if (VLO && values) put_v(buf + SIDE, i, u4_t{});
       }
     }
     if (keys && w.ok && (unsigned)x.rs < (unsigned)a.res.rows && w.rg == o >> a.kg_shift) {  // rare: an open K group
@@ -206,8 +226,8 @@ __device__ __forceinline__ Row row_of(const PrefixArgs& a, int h, int r) {
 }
 
 // The row's query as fragments: 16 bytes at a time, all requested together.
-template <int D, int NKB, bool QLO, bool PLO>
-__device__ __forceinline__ void load_query(Rows<D, false, NKB, 2, QLO, PLO>& w, const PrefixArgs& a, const Row& row, int hh) {
+template <int D, int NKB, bool QLO, bool PLO, bool VLO>
+__device__ __forceinline__ void load_query(Rows<D, false, NKB, 2, QLO, PLO, VLO>& w, const PrefixArgs& a, const Row& row, int hh) {
   constexpr int NS = D / 16, QW = QLO ? 2 : 1;
   w.set_scale(a.scale_log2);
   const uint8_t* src = (const uint8_t*)a.q + (row.q_row * a.q_s0 + (long)row.qh * a.q_s1 + 8 * hh) * (2 * QW);
@@ -249,8 +269,8 @@ __device__ __forceinline__ void mask_tail(f16v_t* s, int left, int hh) {
 }
 
 // The wave's rows out: range z's partial ones, or normalized ones with their log-sum-exp.
-template <int D, int NKB, bool QLO, bool PLO>
-__device__ __forceinline__ void write_rows(Rows<D, false, NKB, 2, QLO, PLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
+template <int D, int NKB, bool QLO, bool PLO, bool VLO>
+__device__ __forceinline__ void write_rows(Rows<D, false, NKB, 2, QLO, PLO, VLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
   const float l = halves_sum(w.l);
   asm volatile("" : "+v"(r));  // the row's place is found again, not kept through the loop
   const Row row = row_of(a, h, r);
@@ -274,8 +294,8 @@ __device__ __forceinline__ void write_rows(Rows<D, false, NKB, 2, QLO, PLO>& w, 
 }
 
 // The wave's rows as range z's partial ones in the workspace are: what write_rows left there.
-template <int D, int NKB, bool QLO, bool PLO>
-__device__ __forceinline__ void resume_rows(Rows<D, false, NKB, 2, QLO, PLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
+template <int D, int NKB, bool QLO, bool PLO, bool VLO>
+__device__ __forceinline__ void resume_rows(Rows<D, false, NKB, 2, QLO, PLO, VLO>& w, const PrefixArgs& a, int h, int r, int z, int hh) {
   const Row row = row_of(a, h, r);
   if (!row.live) return;
   const long pr = ((long)z * a.n + row.t) * a.hq + row.qh;
@@ -304,13 +324,13 @@ __device__ __forceinline__ void write_suffix(const PrefixArgs& a) {
 
 }  // namespace
 
-template <int D, bool QLO, int WAVES, bool PLO>
+template <int D, bool QLO, int WAVES, bool PLO, bool VLO>
 __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) void prefix_kernel(PrefixArgs a) {
   static_assert(WAVES == 4 || WAVES == 8, "a thread takes its items' K and V, or one of them");
   constexpr bool BOTH = WAVES == 4;
   constexpr int KEYS = 8192 / D;           // keys per step: 256 items
   constexpr int NKB = KEYS >= 64 ? 2 : 1;  // 32-key blocks per softmax update
-  using I = Items<D, KEYS>;
+  using I = Items<D, KEYS, VLO>;
   constexpr int SIDE = I::SIDE;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
@@ -335,7 +355,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
   }
   const int r = (tile * WAVES + wave) * 32 + j;
   const bool active = (tile * WAVES + wave) * 32 < (int)a.n * a.gqa;
-  Rows<D, false, NKB, 2, QLO, PLO> w;
+  Rows<D, false, NKB, 2, QLO, PLO, VLO> w;
   load_query(w, a, row_of(a, h, r), hh);
   w.clear();
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
@@ -357,9 +377,9 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
   for (int step = 0; step < n_steps; ++step) {
     __syncthreads();  // every wave is done with the step before (eight waves: and this one is there)
     const int put = BOTH ? step : step + 1;
-    const uint32_t buf = BOTH ? 0u : (uint32_t)((step & 1) * 3 * SIDE);
+    const uint32_t buf = BOTH ? 0u : (uint32_t)((step & 1) * I::STEP);
     if (put < n_steps) {
-      it.store(lds + (BOTH ? 0 : (put & 1) * 3 * SIDE), put, head, raw, keys, values, BOTH);
+      it.store(lds + (BOTH ? 0 : (put & 1) * I::STEP), put, head, raw, keys, values, BOTH);
       if (BOTH) __syncthreads();
       fetch(put + 1);
     }
@@ -374,7 +394,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 256 || (QLO && D == 128) ? 1 : 2) 
       if (left < 32 * NKB) mask_tail<NKB>(s, left, hh);
       w.rescale(w.top(s));
       w.template weights<false, SIDE>(s, p, 0, s);
-      w.template values<false>(p, v_lane + buf + sb * 2 * D, s);
+      w.template values<false, SIDE>(p, v_lane + buf + sb * 2 * D, s);
     }
   }
   write_rows(w, a, h, r, z, hh);
@@ -386,28 +406,28 @@ __device__ __forceinline__ int range_end(const PrefixArgs& a, int z) {
   return z == a.ranges - 1 ? a.len : min(a.len, (z + 1) * a.per);
 }
 
-// One workgroup per (64-key tile of the slab, KV head): its K hi, K lo and V into the workspace. A
-// range's tiles of the slab lie behind one another.
-template <int D>
-__global__ __launch_bounds__(256) void prefix_pack_kernel(PrefixArgs a) {
-  using I = Items<D, kPackKeys>;
+// One workgroup per (64-key tile of the slab, KV head, range): its sides into the workspace. A range's
+// tiles of the slab lie behind one another. Bound by memory: 64 registers, eight waves a SIMD.
+template <int D, bool VLO>
+__global__ __launch_bounds__(256, 8) void prefix_pack_kernel(PrefixArgs a) {
+  using I = Items<D, kPackKeys, VLO>;
   write_suffix(a);
   const int h = (int)(blockIdx.x % (unsigned)a.L.H), tile = (int)(blockIdx.x / (unsigned)a.L.H);
-  const int tiles = a.seg / kPackKeys, z = tile / tiles;
-  const int begin = range_begin(a, z) + a.slab * a.seg + tile % tiles * kPackKeys, end = range_end(a, z);
+  const int z = blockIdx.y, begin = range_begin(a, z) + a.slab * a.seg + tile * kPackKeys, end = range_end(a, z);
   if (begin >= end) return;
   const I it(a, h, begin, end - begin < kPackKeys ? end : begin + kPackKeys, (int)threadIdx.x);
   if (4 * it.quad >= kPackKeys) return;  // head size 64: half of the threads
   Raw raw;
   const Head head = it.load_head(it.load_blk(0));
   it.load(0, head, raw, true, true, true);
-  it.store(a.pack + ((long)tile * a.L.H + h) * (3 * I::SIDE), 0, head, raw, true, true, true);
+  it.store(a.pack + ((long)(z * (a.seg / kPackKeys) + tile) * a.L.H + h) * I::STEP, 0, head, raw, true, true, true);
 }
 
-template <int D, bool PLO>
+template <int D, bool PLO, bool VLO>
 __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   constexpr int WAVES = 8, KEYS = kPackKeys, NKB = 2, SIDE = KEYS * D * 2;
-  constexpr int KDMA = 2 * SIDE / 1024 / WAVES, VDMA = SIDE / 1024 / WAVES;
+  constexpr int VSIDE = (VLO ? 2 : 1) * SIDE, STEP = 2 * SIDE + VSIDE;
+  constexpr int KDMA = 2 * SIDE / 1024 / WAVES, VDMA = VSIDE / 1024 / WAVES;
   // LDS: the keys (hi, lo) of two steps, then the values of two.
   constexpr int V0 = 4 * SIDE;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -419,11 +439,11 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   const int n_steps = k_end > k_begin ? (k_end - k_begin + KEYS - 1) / KEYS : 0;
   if (a.slab > 0 && n_steps == 0) return;  // the rows are as the slabs before left them
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  const uint8_t* tiles = a.pack + ((long)z * (a.seg / KEYS) * a.L.H + h) * (3 * SIDE);
+  const uint8_t* tiles = a.pack + ((long)z * (a.seg / KEYS) * a.L.H + h) * STEP;
   auto issue = [&](int step, bool val) __attribute__((always_inline)) {
     const int n = val ? VDMA : KDMA;
-    const uint8_t* from = uniform_ptr(tiles + (long)step * a.L.H * (3 * SIDE) + (val ? 2 * SIDE : 0) + 1024 * n * wave);
-    const uint32_t to = lds0 + (uint32_t)((val ? V0 + (step & 1) * SIDE : (step & 1) * 2 * SIDE) + 1024 * n * wave);
+    const uint8_t* from = uniform_ptr(tiles + (long)step * a.L.H * STEP + (val ? 2 * SIDE : 0) + 1024 * n * wave);
+    const uint32_t to = lds0 + (uint32_t)((val ? V0 + (step & 1) * VSIDE : (step & 1) * 2 * SIDE) + 1024 * n * wave);
 #pragma unroll
     for (int i = 0; i < n; ++i) dma16(from, 1024 * i + 16 * lane, to + 1024 * i);
   };
@@ -434,7 +454,7 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
   }
   const int r = (tile * WAVES + wave) * 32 + j;
   const bool active = (tile * WAVES + wave) * 32 < (int)a.n * a.gqa;
-  Rows<D, false, NKB, 2, false, PLO> w;
+  Rows<D, false, NKB, 2, false, PLO, VLO> w;
   load_query(w, a, row_of(a, h, r), hh);
   w.clear();
   if (a.slab > 0) resume_rows<D>(w, a, h, r, z, hh);
@@ -455,7 +475,7 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
     w.rescale(mt);
     u4_t p[w.PW];
     w.template weights<true, SIDE>(cur, p, k_lane + (uint32_t)(((step + 1) & 1) * 2 * SIDE), nxt);
-    mt = w.template values<true>(p, v_lane + (uint32_t)((step & 1) * SIDE), nxt);
+    mt = w.template values<true, SIDE>(p, v_lane + (uint32_t)((step & 1) * VSIDE), nxt);
     if (tail && step + 2 == n_steps) {
       mask_tail<NKB>(nxt, tail, hh);
       mt = w.top(nxt);
@@ -481,59 +501,60 @@ __global__ __launch_bounds__(512, 2) void prefix_flash_kernel(PrefixArgs a) {
     w.rescale(mt);
     u4_t p[w.PW];
     w.template weights<false, SIDE>(s0, p, 0, s0);
-    w.template values<false>(p, v_lane + (uint32_t)((step & 1) * SIDE), s0);
+    w.template values<false, SIDE>(p, v_lane + (uint32_t)((step & 1) * VSIDE), s0);
   } else {
     for (int step = 0; step < n_steps; ++step) advance(step);
   }
   write_rows(w, a, h, r, z, hh);
 }
 
-template <int D, bool QLO, int WAVES, bool PLO>
+template <int D, bool QLO, int WAVES, bool PLO, bool VLO>
 static hipError_t launch_t(const PrefixArgs& a, hipStream_t s) {
-  constexpr int lds = (WAVES == 8 ? 2 : 1) * 3 * 8192 * 2;
+  constexpr int lds = (WAVES == 8 ? 2 : 1) * Items<D, 8192 / D, VLO>::STEP;
   static std::atomic<uint64_t> attr_done{0};
-  const hipError_t e = ensure_lds_limit((const void*)prefix_kernel<D, QLO, WAVES, PLO>, lds, &attr_done);
+  const hipError_t e = ensure_lds_limit((const void*)prefix_kernel<D, QLO, WAVES, PLO, VLO>, lds, &attr_done);
   if (e != hipSuccess) return e;
   constexpr int rows = 32 * WAVES;
   const dim3 grid((unsigned)((a.n * a.gqa + rows - 1) / rows * a.L.H), (unsigned)a.ranges);
-  hipLaunchKernelGGL((prefix_kernel<D, QLO, WAVES, PLO>), grid, dim3(64 * WAVES), lds, s, a);
+  hipLaunchKernelGGL((prefix_kernel<D, QLO, WAVES, PLO, VLO>), grid, dim3(64 * WAVES), lds, s, a);
   return hipGetLastError();
 }
 
-template <int D, bool PLO>
+template <int D, bool PLO, bool VLO>
 static hipError_t launch_packed(const PrefixArgs& a, hipStream_t s) {
-  constexpr int lds = 6 * kPackKeys * D * 2;
+  constexpr int lds = (VLO ? 8 : 6) * kPackKeys * D * 2;
   static std::atomic<uint64_t> attr_done{0};
-  hipError_t e = ensure_lds_limit((const void*)prefix_flash_kernel<D, PLO>, lds, &attr_done);
+  hipError_t e = ensure_lds_limit((const void*)prefix_flash_kernel<D, PLO, VLO>, lds, &attr_done);
   if (e != hipSuccess) return e;
-  const unsigned packs = (unsigned)((long)a.ranges * (a.seg / kPackKeys) * a.L.H);
+  const dim3 packs((unsigned)((long)(a.seg / kPackKeys) * a.L.H), (unsigned)a.ranges);
   const dim3 grid((unsigned)((a.n * a.gqa + 255) / 256 * a.L.H), (unsigned)a.ranges);
   PrefixArgs b = a;
   for (int from = 0; from < a.per; from += a.seg, ++b.slab) {
-    hipLaunchKernelGGL(prefix_pack_kernel<D>, dim3(packs), dim3(256), 0, s, b);
+    hipLaunchKernelGGL((prefix_pack_kernel<D, VLO>), packs, dim3(256), 0, s, b);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL((prefix_flash_kernel<D, PLO>), grid, dim3(512), lds, s, b);
+    hipLaunchKernelGGL((prefix_flash_kernel<D, PLO, VLO>), grid, dim3(512), lds, s, b);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     b.suffix = nullptr;  // written by the first
   }
   return hipSuccess;
 }
 
-template <int D, bool PLO>
+template <int D, bool PLO, bool VLO>
 static hipError_t launch_16(const PrefixArgs& a, hipStream_t s) {
-  if constexpr (D == 256) return launch_t<D, false, 4, PLO>(a, s);
-  else if (a.pack) return launch_packed<D, PLO>(a, s);
-  else if (prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa, a.len) == 256) return launch_t<D, false, 8, PLO>(a, s);
-  else return launch_t<D, false, 4, PLO>(a, s);
+  if constexpr (D == 256) return launch_t<D, false, 4, PLO, VLO>(a, s);
+  else if (a.pack) return launch_packed<D, PLO, VLO>(a, s);
+  else if (prefix_rows(a.L.D, a.q_dtype, a.n * a.gqa, a.len) == 256) return launch_t<D, false, 8, PLO, VLO>(a, s);
+  else return launch_t<D, false, 4, PLO, VLO>(a, s);
 }
 
 template <int D>
 static hipError_t launch_d(const PrefixArgs& a, hipStream_t s) {
   if (a.q_dtype == ECHOKV_F32) {
     if constexpr (D == 256) return hipErrorInvalidValue;  // its registers do not fit: attend_any.hip
-    else return launch_t<D, true, 4, true>(a, s);
+    else return a.exact ? launch_t<D, true, 4, true, true>(a, s) : launch_t<D, true, 4, true, false>(a, s);
   }
-  return a.q_dtype == ECHOKV_F16 ? launch_16<D, true>(a, s) : launch_16<D, false>(a, s);
+  if (a.exact) return launch_16<D, true, true>(a, s);
+  return a.q_dtype == ECHOKV_F16 ? launch_16<D, true, false>(a, s) : launch_16<D, false, false>(a, s);
 }
 
 hipError_t launch_prefix(const PrefixArgs& a, hipStream_t s) {

@@ -111,9 +111,10 @@ __device__ __forceinline__ h8_t v_read(uint32_t at, int ks) {
 // go between the score products of step i + 1, whose maxima go between the value products of
 // step i. Scheduling fences hold that order.
 //
-// PARTS: keys as one matrix or as hi + lo, `side` bytes apart. QLO: the queries as hi + lo too, PLO:
-// the weights as float16 hi + lo.
-template <int D, bool BF, int NKB, int PARTS, bool QLO, bool PLO = false>
+// PARTS: keys as one matrix or as hi + lo, `SIDE` bytes apart. QLO: the queries as hi + lo too, PLO:
+// the weights as float16 hi + lo, VLO: the values as hi + lo like the keys (the product of the two low
+// parts, 2^-22 of theirs, is left out).
+template <int D, bool BF, int NKB, int PARTS, bool QLO, bool PLO = false, bool VLO = false>
 struct Rows {
   static constexpr int NS = D / 16, NDB = D / 32;
   static constexpr int NP = 8 * NKB;  // pairs of scores a lane
@@ -238,10 +239,10 @@ struct Rows {
   }
   // O^T += V^T P^T over the values at LDS address v (v_at's lane offset included); returns top() of
   // `next`, taken along.
-  template <bool NEXT>
+  template <bool NEXT, int SIDE = 0>
   __device__ __forceinline__ float values(const u4_t* p, uint32_t v, const f16v_t* next) {
-    constexpr int VU = 2 * NKB * NDB;  // 16 keys x 32 channels each
-    auto load = [&](int u) { return v_read<D>(v ^ 64 * (u % NDB), u / NDB); };
+    constexpr int VP = VLO ? 2 : 1, VU = 2 * NKB * NDB * VP;  // 16 keys x 32 channels of a part each
+    auto load = [&](int u) { return v_read<D>((v ^ 64 * (u / VP % NDB)) + u % VP * SIDE, u / VP / NDB); };
     h8_t f[RING];
     float x = -kInf;
 #pragma unroll
@@ -250,8 +251,11 @@ struct Rows {
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
       if (u + AHEAD < VU) f[(u + AHEAD) % RING] = load(u + AHEAD);
-      acc[u % NDB] = mma<BF>(f[u % RING], __builtin_bit_cast(h8_t, p[u / NDB]), acc[u % NDB]);
-      if constexpr (PLO) acc[u % NDB] = mma<BF>(f[u % RING], __builtin_bit_cast(h8_t, p[NW + u / NDB]), acc[u % NDB]);
+      const int db = u / VP % NDB, ks = u / VP / NDB;
+      acc[db] = mma<BF>(f[u % RING], __builtin_bit_cast(h8_t, p[ks]), acc[db]);
+      if constexpr (PLO) {
+        if (u % VP == 0) acc[db] = mma<BF>(f[u % RING], __builtin_bit_cast(h8_t, p[NW + ks]), acc[db]);
+      }
       if constexpr (NEXT) {
 #pragma unroll
         for (int n = u * NP / VU; n < (u + 1) * NP / VU; ++n)

@@ -10,6 +10,14 @@ takes vLLM's ``common_prefix_len`` and does not use it (``echokv_vllm/backend.py
 The prefix is cut into ranges by the number of query rows, so a sequence's result depends on
 its batch through float rounding (``decode_attention`` alone is batch-invariant).
 
+Precision: scores, maxima, sums and outputs are float32. Into float16 and float32 outputs
+``shared_prefix_decode`` holds keys, values and weights as exact float16 parts, as
+``decode_attention`` does. Into bfloat16 outputs, for speed, the prefix's values and (bfloat16
+queries) weights are rounded to float16 once each: together at most 2^-10 of the sum of weight x
+|value|, where the output's own rounding is 2^-8. ``prefix_attention`` rounds the values to float16
+once (2^-11, as the chunked prefill's kernels), and for bfloat16 queries the weights too. The
+32-bit kernels round nothing.
+
 Kernels: ``echokv_amd/csrc/shared.hip`` (head sizes 64, 128 and 256; queries and keys there are
 float16 parts, so both are to stay within float16's range, as in ``decode_attention``), and
 ``echokv_amd/csrc/attend_any.hip`` (32-bit arithmetic for every other layout, and the join), through
@@ -148,7 +156,9 @@ def shared_prefix_decode(store, query: torch.Tensor, block_table: torch.Tensor, 
     ``prefix_len`` (length 0: graph padding) leaves its row untouched. ``num_splits`` and
     ``blocks_per_split`` (default ``suffix_blocks``) cut the tokens behind the prefix.
     ``workspace``: uint8, ``shared_workspace_bytes(...)``; by default the call allocates it. A prefix
-    of 0 tokens is plain decode."""
+    of 0 tokens is plain decode. Short prefixes (below about 1024 tokens) take no less time here than
+    in ``decode_attention``: two launches more, and little to share. Outputs in bfloat16 round the
+    prefix's weights and values once more than ``decode_attention`` (see the module)."""
     prefix_len = int(prefix_len)
     if prefix_len == 0:
         return dec.decode_attention(store, query, block_table, seq_lens, softmax_scale,

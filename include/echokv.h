@@ -301,7 +301,8 @@ int echokv_prompt(const void* query, int64_t q_s0, int64_t q_s1, const void* key
  * ceil(prefix_len / block_size) entries). part (float32, row q_rows[i], strides p_s0 / p_s1) gets
  * the normalized rows and lse (float [rows, num_q_heads]) their log2-domain log-sum-exp (zeros
  * and -inf for prefix_len 0). workspace: echokv_prefix_workspace(...) bytes, 16-byte aligned; it
- * serves every query type and grows with n, with prefix_len by 128 MiB at most.
+ * serves every query type and grows with n, with prefix_len by 128 MiB at most. Values are rounded to
+ * float16 once, as in echokv_prefill, and for bfloat16 queries the weights.
  * Results depend on n through float rounding (the keys are cut into ranges by it).
  * No counterpart in the reference. */
 int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t n, int64_t prefix_len);
@@ -318,7 +319,9 @@ int echokv_prefix(const echokv_layout* L, const uint8_t* pages, const int64_t* b
  * tier and tier_mask; num_splits cuts the tokens behind the prefix), and both are joined into
  * out[q_rows[i]]. Sequences shorter than prefix_len (length 0: graph padding) leave their row
  * untouched. workspace: echokv_shared_decode_workspace(...) bytes, 16-byte aligned. Results
- * depend on num_seqs through float rounding. No counterpart in the reference, whose builder
+ * depend on num_seqs through float rounding. Into float16 and float32 weights and values are exact
+ * float16 parts, as in echokv_decode; into bfloat16 the prefix's are rounded to float16 once each (the
+ * weights for bfloat16 queries): at most 2^-10 of the sum of weight x |value|. No counterpart in the reference, whose builder
  * leaves its common_prefix_len unused (echokv_vllm/backend.py:337-496). */
 int64_t echokv_shared_decode_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t num_seqs,
                                        int64_t prefix_len, int32_t num_splits);
