@@ -114,6 +114,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         _lib.require_current(query)
         plan = build_prompt_plan(prefill, hq // h, d, query.device)
     part, p_lse = prefix if prefix is not None else (None, None)
+    if (part is None) != (p_lse is None):
+        raise ValueError("a prefix is rows and their log-sum-exp, both")
     _lib.require_current(query, key, value, output, lse, part, p_lse, plan.tiles)
     if plan.gqa != hq // h or plan.head_size != d:
         raise ValueError("the plan was built for other heads")

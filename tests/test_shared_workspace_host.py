@@ -54,6 +54,16 @@ def test_suffix_rows_are_aligned(h, gqa, seqs, tokens, ranges):
     assert size == lengths + ranges * rows * d * 4 + pairs + splits * rows * d * 4 + splits * rows * 8
 
 
+def test_prompt_refuses_half_a_prefix():
+    from echokv_amd.kernels.prompt import build_prompt_plan, prompt_attention
+
+    q, k = torch.zeros(4, 8, 128), torch.zeros(4, 2, 128)
+    plan = build_prompt_plan([(0, 4)], 4, 128, torch.device("cpu"))
+    for prefix in ((torch.zeros(4, 8, 128), None), (None, torch.zeros(4, 8))):
+        with pytest.raises(ValueError, match="prefix"):
+            prompt_attention(q, k, k, q, (), 0.1, plan=plan, prefix=prefix)
+
+
 # ---- the backend's steps --------------------------------------------------------------------
 
 def _builder(monkeypatch):
