@@ -121,12 +121,15 @@ struct Items {
       }
     }
   }
-  // Eight channels as float16 hi + lo, at `buf` + `at` and SIDE behind it.
+  // Eight channels as float16 hi + lo, at `buf` + `at` and SIDE behind it. CLAMP: statistics rounded
+  // up can take the largest float16 value past its type (65504 in INT4 to 65536); lo holds the rest.
+  template <bool CLAMP = false>
   __device__ __forceinline__ void put2(uint8_t* buf, int at, const float* x8) const {
     u4_t hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const h2_t p = {(_Float16)x8[2 * e], (_Float16)x8[2 * e + 1]};
+      auto first = [](float x) { return (_Float16)(CLAMP ? __builtin_amdgcn_fmed3f(x, -65504.f, 65504.f) : x); };
+      const h2_t p = {first(x8[2 * e]), first(x8[2 * e + 1])};
       hi[e] = __builtin_bit_cast(uint32_t, p);
       lo[e] = pack2<false>(x8[2 * e] - (float)p[0], x8[2 * e + 1] - (float)p[1]);
     }
@@ -175,7 +178,7 @@ struct Items {
             float x8[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x8[e] = __builtin_fmaf((float)c[e >> 1][e & 1], (float)vs[0], (float)vm[0]);
-            put2(buf + 2 * SIDE, v_slot(i), x8);
+            put2<true>(buf + 2 * SIDE, v_slot(i), x8);
           } else {
             u4_t v;
 #pragma unroll

@@ -22,7 +22,7 @@ TWO_PARTS = 2.0 ** -21  # a float16 hi + lo pair: 2^-22, the product of two low 
 
 
 class Probe:
-    def __init__(self, device, d, gqa, seqs, prefix, whole_values, h=2, bs=16, vg=32, seed=0):
+    def __init__(self, device, d, gqa, seqs, prefix, whole_values, h=2, bs=16, vg=32, seed=0, tier=4, largest=0.0):
         g = torch.Generator(device=device)
         g.manual_seed(seed)
         rng = np.random.default_rng(seed)
@@ -44,9 +44,12 @@ class Probe:
         if whole_values:  # 0 to 15, both in every V group: exact in INT4 and in float16
             v = torch.randint(0, 16, v.shape, device=device, generator=g).float()
             v[:, :, ::vg], v[:, :, 1::vg] = 0.0, 15.0
+        if largest:  # both signs in every V group
+            v = largest * (2 * torch.rand(v.shape, device=device, generator=g) - 1)
+            v[:, :, ::vg], v[:, :, 1::vg] = -largest, largest
         slots = np.concatenate([table[0][np.arange(prefix) // bs] * bs + np.arange(prefix) % bs,
                                 (table[:, -1:] * bs + np.arange(tail)).reshape(-1)])
-        self.store.write(k.half(), v.half(), torch.from_numpy(slots), 4)
+        self.store.write(k.half(), v.half(), torch.from_numpy(slots), tier)
         self.table_np, self.table = table, torch.from_numpy(table).to(device, torch.int32)
         self.lens = torch.full((seqs,), prefix + tail, device=device)
         self.q = torch.zeros(seqs, h * gqa, d, device=device)
@@ -101,3 +104,20 @@ def test_prefix_weights(device, d, gqa, seqs, prefix, dtype):
         r = expect(c, q, i, prefix)
         check(part[i : i + 1], r, weight=unit(F16) if dtype == BF16 else TWO_PARTS)
         assert float((lse[i] - r.lse).abs().max()) <= r.lse_bound()
+
+
+@pytest.mark.parametrize("d,gqa,seqs,prefix", [(128, 4, 3, 512), (256, 4, 3, 512), (64, 8, 20, 6400), (128, 4, 200, 4096)])
+@pytest.mark.parametrize("tier", [2, 4, 8])
+def test_the_largest_values(device, d, gqa, seqs, prefix, tier):
+    """Values of -65504 and 65504 in every V group: dequantized (65536 in INT4) they can pass float16."""
+    print(f"[precision] largest {d} {gqa} {seqs} {prefix} INT{tier}", flush=True)
+    c = Probe(device, d, gqa, seqs, prefix, whole_values=False, tier=tier, largest=65504.0, seed=d + seqs)
+    q = c.q.half()
+    got = shared_prefix_decode(c.store, q, c.table, c.lens, prefix, 1.0, tier=tier)
+    torch.cuda.synchronize()
+    passed = False
+    for i in sorted({0, 1, seqs - 1}):
+        r = expect(c, q, i, prefix + 5)
+        passed = passed or r.vmax > 65504
+        check(got[i : i + 1], r, weight=TWO_PARTS, value=TWO_PARTS)
+    assert passed or tier != 4
