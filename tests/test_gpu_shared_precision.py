@@ -38,8 +38,10 @@ class Probe:
         n = prefix + tail * seqs
         k, v = (torch.randn(n, h, d, device=device, generator=g) for _ in range(2))
         k[:, :, 0] = 0.0
-        # One target a K group at most: its value is 15 steps of the group, the others' 0.
-        self.targets = np.sort(rng.choice(shared, TARGETS, replace=False)) * bs + rng.integers(0, bs, TARGETS)
+        # One target a K group at most: its value is 15 steps of the group, the others' 0. All in 128 aligned
+        # keys, so in one range: alone in its range a target's weight is 1, which every type holds.
+        groups = rng.integers(prefix // 128) * (128 // bs) + rng.choice(128 // bs, TARGETS, replace=False)
+        self.targets = np.sort(groups) * bs + rng.integers(0, bs, TARGETS)
         k[torch.from_numpy(self.targets).to(device), :, 0] = 30 + torch.rand(TARGETS, h, device=device, generator=g)
         if whole_values:  # 0 to 15, both in every V group: exact in INT4 and in float16
             v = torch.randint(0, 16, v.shape, device=device, generator=g).float()
