@@ -29,7 +29,7 @@
 // maximum and sum that the slab before left in its workspace row.
 //
 // Measured (8 KV heads of GQA 4, D 128): 64 sequences (256 rows) behind 4096 INT4 keys 23 us in
-// prefix_kernel, of which 16 ranges' partial rows (17 MB) are 3 at the rate of a copy and the loads'
+// prefix_kernel (27 with VLO), of which 16 ranges' partial rows (17 MB) are 3 at the rate of a copy and the loads'
 // chain (block id, header, codes) with four steps the rest. 8065 bfloat16 rows behind 8192: pack 16
 // us, then flash 1.36 to 1.44 ms, bound by the matrix cores: 0.76 to 0.80 PFLOP/s of the formula's
 // products, 1.14 to 1.19 of those made (a key's two parts make the scores twice the work), MFMA

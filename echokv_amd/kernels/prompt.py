@@ -92,7 +92,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     prompt, float32 ``[T, Hq, D]`` with its log-sum-exp ``[T, Hq]``
     (``kernels.shared.prefix_attention``), joined with the result; a row whose ``part_lse`` is -inf
     has none. 16-bit rows of head size 64, 128 or 256, 16-byte aligned, have the same bits whatever
-    else the step holds; in the 32-bit kernels (every other case) they depend on the step's size
+    else the step holds, and each of their softmax weights is rounded to the inputs' type once (of
+    weight x |value| bfloat16 2^-8, float16 2^-11), whatever the output's type; in the 32-bit kernels
+    (every other case) nothing is held in fewer than 32 bits, and the bits depend on the step's size
     through float rounding."""
     if plan is None and not prefill:
         return

@@ -16,7 +16,7 @@ Precision: scores, maxima, sums and outputs are float32. Into float16 and float3
 queries) weights are rounded to float16 once each: together at most 2^-10 of the sum of weight x
 |value|, where the output's own rounding is 2^-8. ``prefix_attention`` rounds the values to float16
 once (2^-11, as the chunked prefill's kernels), and for bfloat16 queries the weights too. The
-32-bit kernels round nothing.
+32-bit kernels hold everything in 32 bits.
 
 Kernels: ``echokv_amd/csrc/shared.hip`` (head sizes 64, 128 and 256; queries and keys there are
 float16 parts, so both are to stay within float16's range, as in ``decode_attention``), and
