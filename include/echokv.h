@@ -301,8 +301,9 @@ int echokv_prompt(const void* query, int64_t q_s0, int64_t q_s1, const void* key
  * ceil(prefix_len / block_size) entries). part (float32, row q_rows[i], strides p_s0 / p_s1) gets
  * the normalized rows and lse (float [rows, num_q_heads]) their log2-domain log-sum-exp (zeros
  * and -inf for prefix_len 0). workspace: echokv_prefix_workspace(...) bytes, 16-byte aligned; it
- * serves every query type and grows with n, with prefix_len by 128 MiB at most. Values are rounded to
- * float16 once, as in echokv_prefill, and for bfloat16 queries the weights.
+ * serves every query type and holds partial rows (by n) and at most 128 MiB of dequantized keys,
+ * however long the prefix is. Values are rounded to float16 once, as in echokv_prefill, and for
+ * bfloat16 queries the weights.
  * Results depend on n through float rounding (the keys are cut into ranges by it).
  * No counterpart in the reference. */
 int64_t echokv_prefix_workspace(const echokv_layout* L, int32_t num_q_heads, int64_t n, int64_t prefix_len);
