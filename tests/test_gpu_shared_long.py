@@ -59,3 +59,34 @@ def test_decode_behind_several_slabs(device):
         k, v = c.tokens(i, c.lens[i])
         check(out[i : i + 1], Rows(q[i : i + 1], k, v, [c.lens[i]], c.d ** -0.5), **BOUND)
     assert (out[5] == 9).all() and (out[7] == 9).all()
+
+
+def test_slabs_in_a_graph(device):
+    """Captured and replayed, the lengths changing, with eager calls between: every replay equals the eager
+    result bit for bit."""
+    print("[slabs] graph", flush=True)
+    c = Cache(device, 32000, [3, 70] * 70, h=8, bs=64, kg=32)
+    q = c.queries(140, 4, F16)
+    lens = torch.tensor(c.lens, device=device)
+    rows = torch.arange(139, 0, -1, device=device)
+    out, part, lse = torch.zeros_like(q), torch.zeros_like(q, dtype=torch.float32), torch.zeros(140, 32, device=device)
+
+    def call(o, p, x):
+        shared_prefix_decode(c.store, q, c.table, lens, c.prefix, c.d ** -0.5, out=o, tier=4)
+        prefix_attention(c.store, q, c.blocks, c.prefix, c.d ** -0.5, part=p, lse=x, q_rows=rows)
+
+    call(out, part, lse)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out, part, lse)
+    for rep in range(3):
+        lens.copy_(torch.tensor([max(c.prefix, n - 9 * rep) for n in c.lens], device=device))
+        for t in (out, part, lse):
+            t.zero_()
+        g.replay()
+        eager = [torch.zeros_like(t) for t in (out, part, lse)]
+        call(*eager)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((out, part, lse), eager)), rep
+        assert (part[0] == 0).all() and (out[0] != 0).any()
